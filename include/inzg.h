@@ -28,8 +28,11 @@
 extern "C" {
 #endif
 
-/* tensor type ids, as in the reference's GGUF (src/quant.h:25-37) */
+/* tensor type ids, as in the reference's GGUF (src/quant.h:25-37; F32 and BF16 are the GGUF container's) */
+#define INZG_T_F32 0
 #define INZG_T_F16 1
+#define INZG_T_BF16 30
+#define INZG_T_E4M3 110  /* 8-bit floating point, 4 exponent and 3 mantissa bits, largest value 448 (an id of this ABI) */
 #define INZG_T_Q4L 102
 #define INZG_T_Q8G 103
 
@@ -243,8 +246,104 @@ INZG_EXPORT inzg_status inzg_hc_out(inzg_ctx *ctx, int n, float *X_dev, const fl
  * is updated in place. */
 INZG_EXPORT inzg_status inzg_moe_block_hc(inzg_ctx *ctx, int layer, int n, float *X_dev, const inzg_moe_opts *opt);
 
+/* ---- Experts in 8-bit floating point (e4m3 with one fp32 scale per block of 128) or bf16 / f16: the operators of an MoE
+ * layer whose weights are not the engine's Q4L / Q8G blobs, e.g. those of an FP8 checkpoint used as they are. Together
+ * with inzg_route (sel, w) and inzg_combine (slots -> y) they are the layer:
+ *   inzg_rmsnorm_q8 -> inzg_expert_lists -> inzg_grouped_matmul (gate|up, rows gathered) -> inzg_silu_mul_q8
+ *   -> inzg_grouped_matmul (down, weighted rows into the tokens' slots) -> inzg_combine
+ * and inzg_matmul_q8 is the dense product of the same activations.
+ *
+ * All pointers are device pointers of the context's device; calls are ordered on `stream` (NULL = the context's
+ * stream), return without synchronising, allocate nothing, keep nothing between calls, may be captured into a CUDA
+ * graph, may overlap on different streams, and leave the caller's current device as it was. They use only the
+ * context's device, stream and error word, never its configured sizes. A pitch (`ld...`) is the distance of two
+ * rows in elements; 0 means contiguous rows. Zero rows are no work, not an error; only the elements named below are
+ * written. Outputs must not overlap inputs except where said.
+ *
+ * Quantized rows: value[i][c] = q[i][c] * s[i][c / 128]. The quantizers set, per row and block of 128 columns,
+ * s = max(max |v|, 2^-100) / 448 and q = e4m3(v / s), nearest, ties to even. A NaN stays a NaN in its place; a block
+ * that holds an infinity has an infinite scale and no finite value.
+ *
+ * Device-side checks (an expert id out of range, offsets that are not ascending within the entries, a row index out of
+ * range) never read or write out of range; inzg_device_status reports them once (INZG_DEVICE_CHECK). */
+#define INZG_Q8_BLOCK 128
+#define INZG_MAX_GROUPS 2048
+
+/* RMS norm of rows, with the residual's addition: h = x + res (fp32); sum = h in `type`; v = h / sqrt(mean(h^2) + eps) * w,
+ * from the unrounded h; y = v in `type`; q, s = v quantized. */
+typedef struct {
+    int n, cols, type;                          /* rows, columns (<= 32768); INZG_T_F32, _F16 or _BF16 of x, res, sum, y */
+    const void *x; int64_t ldx;
+    const void *res; int64_t ldres;             /* NULL: no residual */
+    void *sum; int64_t ldsum;                   /* NULL: not written; may be x or res itself (with its pitch) */
+    const float *w;                             /* [cols] */
+    float eps;
+    void *y; int64_t ldy;                       /* NULL: not written */
+    void *q; int64_t ldq;                       /* e4m3; NULL (with s): not written */
+    float *s; int64_t lds;                      /* [n][ceil(cols / 128)] */
+    void *stream;
+} inzg_rmsnorm_q8_args;
+INZG_EXPORT inzg_status inzg_rmsnorm_q8(inzg_ctx *ctx, const inzg_rmsnorm_q8_args *args);
+
+/* SiLU(gate) * up of rows gate|up: v[i][c] = g / (1 + exp(-g)) * u with g = x[i][c], u = x[i][cols + c]; y = v in
+ * `type`; q, s = v quantized. */
+typedef struct {
+    int n, cols, type;                          /* rows, columns of the result; INZG_T_F32, _F16 or _BF16 of x and y */
+    const void *x; int64_t ldx;                 /* [n][2 * cols] */
+    void *y; int64_t ldy;                       /* NULL: not written */
+    void *q; int64_t ldq;                       /* e4m3; NULL (with s): not written */
+    float *s; int64_t lds;                      /* [n][ceil(cols / 128)] */
+    void *stream;
+} inzg_silu_mul_q8_args;
+INZG_EXPORT inzg_status inzg_silu_mul_q8(inzg_ctx *ctx, const inzg_silu_mul_q8_args *args);
+
+/* The entries of n tokens' selections in order of expert, then slot t * topk + k: off [n_expert + 1] (the entries of
+ * expert e are off[e] .. off[e + 1] - 1), rows (the token t of each entry), slots, w_out (w of each entry; NULL with w).
+ * sel [n][topk]; a negative expert is on another rank and not listed, one >= n_expert is a device-side error and not
+ * listed. n_expert <= INZG_MAX_GROUPS. */
+INZG_EXPORT inzg_status inzg_expert_lists(inzg_ctx *ctx, int n, int topk, int n_expert, const int32_t *sel,
+                                          const float *w, int32_t *off, int32_t *rows, int32_t *slots, float *w_out,
+                                          void *stream);
+
+/* out[i][j] = sum over blocks b of a_scale[i][b] * w_scale[j / 128][b] * (sum over the block's k of a[i][k] * w[j][k]),
+ * summed in fp32 and rounded once to out_type. a, w: e4m3, 16-byte aligned, pitches multiples of 16. */
+typedef struct {
+    int m, n, k;
+    const void *a; int64_t lda;                 /* [m][k] */
+    const float *a_scale; int64_t lda_scale;    /* [m][ceil(k / 128)] */
+    const void *w; int64_t ldw;                 /* [n][k] */
+    const float *w_scale;                       /* [ceil(n / 128)][ceil(k / 128)], contiguous */
+    void *out; int64_t ldo; int out_type;       /* [m][n]; INZG_T_F32, _F16 or _BF16 */
+    void *stream;
+} inzg_matmul_q8_args;
+INZG_EXPORT inzg_status inzg_matmul_q8(inzg_ctx *ctx, const inzg_matmul_q8_args *args);
+
+/* Products grouped by expert: for each group g and entry i in off[g] .. off[g + 1] - 1 (off on the device, ascending
+ * from 0 or more to `entries` or less; groups may be empty)
+ *   out[out_rows ? out_rows[i] : i][j] = (out_scale ? out_scale[i] : 1) * sum over k of a[in_rows ? in_rows[i] : i][k] * w[g][j][k]
+ * with the block scales of inzg_matmul_q8 for INZG_T_E4M3; summed in fp32 and rounded once to out_type. a, w 16-byte
+ * aligned, their pitches multiples of 16 bytes. Entries outside the lists, and rows of out that none names, are left as they
+ * were; an entry whose index is out of range is skipped and reported. A row of out named twice holds either value. */
+typedef struct {
+    int type;                                   /* of a and w: INZG_T_E4M3, _BF16 or _F16 */
+    int groups, n, k;                           /* groups <= INZG_MAX_GROUPS */
+    int a_rows, entries, out_rows_n;            /* rows of a; upper bound of off[groups]; rows of out */
+    const void *a; int64_t lda;                 /* [a_rows][k] */
+    const float *a_scale; int64_t lda_scale;    /* [a_rows][ceil(k / 128)]; INZG_T_E4M3 only, else NULL */
+    const void *w; int64_t ldw;                 /* [groups][n][k], group g's row j at w + (g * n + j) * ldw */
+    const float *w_scale;                       /* [groups][ceil(n / 128)][ceil(k / 128)]; INZG_T_E4M3 only, else NULL */
+    const int32_t *off;                         /* [groups + 1] */
+    const int32_t *in_rows, *out_rows;          /* [entries], each optional; without in_rows a_rows >= entries,
+                                                   without out_rows out_rows_n >= entries */
+    const float *out_scale;                     /* [entries], optional */
+    void *out; int64_t ldo; int out_type;       /* [out_rows_n][n]; INZG_T_F32, _F16 or _BF16 */
+    void *stream;
+} inzg_grouped_matmul_args;
+INZG_EXPORT inzg_status inzg_grouped_matmul(inzg_ctx *ctx, const inzg_grouped_matmul_args *args);
+
 /* Waits for `stream` and reports the device-side checks of the calls since the last routing step
- * (INZG_TIMEOUT / INZG_DEVICE_CHECK), including a timed-out expert-parallel exchange. */
+ * (INZG_TIMEOUT / INZG_DEVICE_CHECK), including a timed-out expert-parallel exchange and the checks of the 8-bit
+ * floating point operators since the last report. */
 INZG_EXPORT inzg_status inzg_device_status(inzg_ctx *ctx, void *stream);
 
 /* ---- Expert parallelism with the exchange in the library: peer memory over NVLink / NVSwitch, no collective library.

@@ -10,6 +10,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libinzg.so")
 
 T_F16, T_Q4L, T_Q8G = 1, 102, 103
+T_F32, T_BF16, T_E4M3 = 0, 30, 110
 IO_DEVICE, DUMP_ROUTE, PROFILE, NO_GRAPH, GEMM_SIMT, NO_FUSED = 1, 2, 4, 8, 16, 32
 EP_HANDLE_BYTES = 128  # INZG_EP_HANDLE_BYTES
 N_STAGES = 12
@@ -37,6 +38,37 @@ class Stats(ctypes.Structure):
     _fields_ = [("calls", ctypes.c_uint64), ("tokens", ctypes.c_uint64), ("units", ctypes.c_uint64),
                 ("dec_units", ctypes.c_uint64), ("gemm_units", ctypes.c_uint64), ("pool_bytes", ctypes.c_uint64),
                 ("last_launches", ctypes.c_int)]
+
+
+class RmsnormQ8Args(ctypes.Structure):
+    _fields_ = [("n", ctypes.c_int), ("cols", ctypes.c_int), ("type", ctypes.c_int), ("x", ctypes.c_void_p),
+                ("ldx", ctypes.c_int64), ("res", ctypes.c_void_p), ("ldres", ctypes.c_int64), ("sum", ctypes.c_void_p),
+                ("ldsum", ctypes.c_int64), ("w", ctypes.c_void_p), ("eps", ctypes.c_float), ("y", ctypes.c_void_p),
+                ("ldy", ctypes.c_int64), ("q", ctypes.c_void_p), ("ldq", ctypes.c_int64), ("s", ctypes.c_void_p),
+                ("lds", ctypes.c_int64), ("stream", ctypes.c_void_p)]
+
+
+class SiluMulQ8Args(ctypes.Structure):
+    _fields_ = [("n", ctypes.c_int), ("cols", ctypes.c_int), ("type", ctypes.c_int), ("x", ctypes.c_void_p),
+                ("ldx", ctypes.c_int64), ("y", ctypes.c_void_p), ("ldy", ctypes.c_int64), ("q", ctypes.c_void_p),
+                ("ldq", ctypes.c_int64), ("s", ctypes.c_void_p), ("lds", ctypes.c_int64), ("stream", ctypes.c_void_p)]
+
+
+class MatmulQ8Args(ctypes.Structure):
+    _fields_ = [("m", ctypes.c_int), ("n", ctypes.c_int), ("k", ctypes.c_int), ("a", ctypes.c_void_p),
+                ("lda", ctypes.c_int64), ("a_scale", ctypes.c_void_p), ("lda_scale", ctypes.c_int64),
+                ("w", ctypes.c_void_p), ("ldw", ctypes.c_int64), ("w_scale", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                ("ldo", ctypes.c_int64), ("out_type", ctypes.c_int), ("stream", ctypes.c_void_p)]
+
+
+class GroupedMatmulArgs(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int), ("groups", ctypes.c_int), ("n", ctypes.c_int), ("k", ctypes.c_int),
+                ("a_rows", ctypes.c_int), ("entries", ctypes.c_int), ("out_rows_n", ctypes.c_int), ("a", ctypes.c_void_p),
+                ("lda", ctypes.c_int64), ("a_scale", ctypes.c_void_p), ("lda_scale", ctypes.c_int64),
+                ("w", ctypes.c_void_p), ("ldw", ctypes.c_int64), ("w_scale", ctypes.c_void_p), ("off", ctypes.c_void_p),
+                ("in_rows", ctypes.c_void_p), ("out_rows", ctypes.c_void_p), ("out_scale", ctypes.c_void_p),
+                ("out", ctypes.c_void_p), ("ldo", ctypes.c_int64), ("out_type", ctypes.c_int),
+                ("stream", ctypes.c_void_p)]
 
 
 P, I, U32, U64, I64, F = (ctypes.c_void_p, ctypes.c_int, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_int64,
@@ -75,6 +107,11 @@ SIGNATURES = {
     "inzg_hc_in": (I, [P, I, I, P, P, P, P]),
     "inzg_hc_out": (I, [P, I, P, P, P, P]),
     "inzg_moe_block_hc": (I, [P, I, I, P, ctypes.POINTER(MoeOpts)]),
+    "inzg_rmsnorm_q8": (I, [P, ctypes.POINTER(RmsnormQ8Args)]),
+    "inzg_silu_mul_q8": (I, [P, ctypes.POINTER(SiluMulQ8Args)]),
+    "inzg_expert_lists": (I, [P, I, I, I, P, P, P, P, P, P, P]),
+    "inzg_matmul_q8": (I, [P, ctypes.POINTER(MatmulQ8Args)]),
+    "inzg_grouped_matmul": (I, [P, ctypes.POINTER(GroupedMatmulArgs)]),
     "inzg_gguf_open": (P, [ctypes.c_char_p, ctypes.POINTER(GgufInfo), ctypes.c_char_p, ctypes.c_size_t]),
     "inzg_gguf_get_info": (I, [P, ctypes.POINTER(GgufInfo)]),
     "inzg_gguf_experts": (I, [P, I, ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(U64), ctypes.POINTER(U64)]),

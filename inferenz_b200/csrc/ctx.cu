@@ -165,6 +165,7 @@ struct inzg_ctx {
     cudaStream_t capture_stream = nullptr;
     cudaStream_t side = nullptr;            // branch for the input quantization, joined before the experts
     cudaEvent_t fork = nullptr, join = nullptr;
+    int32_t *op_err = nullptr;  // error word of the 8-bit floating point operators, sticky until inzg_device_status
 };
 
 static const char *kStageNames[INZG_N_STAGES] = {"router_logits", "softmax_topk_route", "act_quant", "route",
@@ -211,7 +212,7 @@ static void free_scratch(inzg_ctx *c) {
                     c->gemm_units, c->gemm_tiles, c->upath, c->eexp, c->ew, c->GU, c->mo, c->dq64, c->dq256, c->dsb64,
                     c->ds256, c->xqe, c->xse, c->sh_cnt, c->sh_off, c->sh_first, c->sh_etok, c->sh_eslot,
                     c->sh_eexp, c->sh_upath, c->sh_units, c->sh_dec, c->sh_gemm, c->sh_tiles, c->sh_meta, c->sh_ew,
-                    c->cmask, c->fused_cnt};
+                    c->cmask, c->fused_cnt, c->op_err};
     for (void *p : ptrs)
         if (p) cudaFree(p);
 }
@@ -307,6 +308,8 @@ inzg_ctx *inzg_create(const inzg_config *cfg, inzg_status *status) {
     c->fused_cnt = dalloc<int32_t>(fused_counter_ints((int)E, 8, (int)H), ok);
     if (ok && cudaMemset(c->fused_cnt, 0, sizeof(int32_t) * fused_counter_ints((int)E, 8, (int)H)) != cudaSuccess)
         ok = false;
+    c->op_err = dalloc<int32_t>(1, ok);
+    if (ok && cudaMemset(c->op_err, 0, sizeof(int32_t)) != cudaSuccess) ok = false;
     if (!ok) {
         free_scratch(c);
         cudaStreamDestroy(c->stream);
@@ -317,6 +320,7 @@ inzg_ctx *inzg_create(const inzg_config *cfg, inzg_status *status) {
     router_set_attributes(cfg->hidden);
     gemv_set_attributes();
     gemm_tc_set_attributes();
+    gmm_set_attributes();
     c->have_tc = make_tma_map_i8(c->map_xqe.bytes, c->xqe, NE, H, 128) && make_tma_map_i8(c->map_dq.bytes, c->dq256, NE, FF, 128);
     for (int i = 0; i <= INZG_N_STAGES; i++) cudaEventCreate(&c->ev[i]);
     cudaStreamCreateWithFlags(&c->capture_stream, cudaStreamNonBlocking);
@@ -1018,6 +1022,19 @@ inzg_status inzg_device_status(inzg_ctx *c, void *stream) {
         if (e != cudaSuccess) return cuda_fail(c, e, "device_status");
         if (ep_err != kErrNone) return fail(c, INZG_TIMEOUT, "expert-parallel exchange: a peer did not arrive in time");
     }
+    int32_t op_err = 0;
+    e = cudaMemcpyAsync(&op_err, c->op_err, sizeof(op_err), cudaMemcpyDeviceToHost, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (e == cudaSuccess && op_err != kErrNone) {
+        e = cudaMemsetAsync(c->op_err, 0, sizeof(int32_t), st);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    }
+    if (e != cudaSuccess) return cuda_fail(c, e, "device_status");
+    if (op_err == kErrTimeout) return fail(c, INZG_TIMEOUT, "grouped_matmul: a device-side wait ran out");
+    if (op_err != kErrNone)
+        return fail(c, INZG_DEVICE_CHECK, op_err == kErrBadExpert ? "expert_lists: an expert id is out of range"
+                                          : op_err == kErrOverflow ? "grouped_matmul: offsets out of order or out of range"
+                                                                   : "grouped_matmul: a row index is out of range");
     return INZG_OK;
 }
 
@@ -1314,6 +1331,14 @@ int inzg__router_view(const inzg_ctx *c, int layer, const void **router, int *de
     *stream = c->stream;
     *meta = c->meta;
     return 1;
+}
+
+// and for ops.cu
+void inzg__op_view(const inzg_ctx *c, int *device, int *num_sms, void **stream, int32_t **err) {
+    *device = c->cfg.device;
+    *num_sms = c->num_sms;
+    *stream = c->stream;
+    *err = c->op_err;
 }
 
 void inzg__set_error(inzg_ctx *c, const char *msg) {

@@ -108,4 +108,13 @@ int launch_fused_decode(const LayerDev &L, int n, int K, const float *x, const f
                         int8_t *xq64, float2 *xsb64, float *GU, int8_t *dq64, float2 *dsb64, float *mo, float *y,
                         int32_t *counters, int num_sms, cudaStream_t st);
 
+// The 8-bit floating point operators (checked arguments; include/inzg.h). err: the context's error word of theirs.
+int launch_rmsnorm_q8(const inzg_rmsnorm_q8_args &args, int num_sms, cudaStream_t st);
+int launch_silu_mul_q8(const inzg_silu_mul_q8_args &args, int num_sms, cudaStream_t st);
+int launch_expert_lists(int n, int topk, int E, const int32_t *sel, const float *w, int32_t *off, int32_t *rows,
+                        int32_t *slots, float *w_out, int32_t *err, cudaStream_t st);
+void gmm_set_attributes();
+// off null: one group of all entries (inzg_matmul_q8); -1: no tensor map for the operands
+int launch_grouped_matmul(const inzg_grouped_matmul_args &G, int num_sms, int32_t *err, cudaStream_t st);
+
 }  // namespace inzg

@@ -1,0 +1,97 @@
+// k_q8.cuh -- element access and the block-of-128 e4m3 quantizer shared by the 8-bit floating point operators, sm_100a.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "../../include/inzg.h"
+
+namespace inzg {
+
+constexpr int kQB = INZG_Q8_BLOCK;  // columns per scale
+constexpr float kE4m3Max = 448.0f;
+constexpr float kAmaxFloor = 7.888609052210118e-31f;  // 2^-100: keeps the scale and its reciprocal normal numbers
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void from_f32(float v, float &o) { o = v; }
+__device__ __forceinline__ void from_f32(float v, __half &o) { o = __float2half_rn(v); }
+__device__ __forceinline__ void from_f32(float v, __nv_bfloat16 &o) { o = __float2bfloat16_rn(v); }
+
+// A thread's chunk: 8 neighbouring elements (16 or 32 bytes), so that a block of 128 columns is 16 lanes of one warp.
+template <class T>
+struct alignas(16) Chunk {
+    T v[8];
+};
+
+// the chunk at p as fp32; VEC: p is 16-byte aligned. `left`: elements of the row from p on (what lies behind reads 0)
+template <class T, bool VEC>
+__device__ __forceinline__ void load_chunk(const T *p, int left, float (&o)[8]) {
+    if (VEC && left >= 8) {
+        Chunk<T> c;
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(c) / 16; i++)
+            reinterpret_cast<uint4 *>(&c)[i] = reinterpret_cast<const uint4 *>(p)[i];
+#pragma unroll
+        for (int i = 0; i < 8; i++) o[i] = to_f32(c.v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) o[i] = i < left ? to_f32(p[i]) : 0.0f;
+    }
+}
+
+template <class T, bool VEC>
+__device__ __forceinline__ void store_chunk(T *p, int left, const float (&v)[8]) {
+    Chunk<T> c;
+#pragma unroll
+    for (int i = 0; i < 8; i++) from_f32(v[i], c.v[i]);
+    if (VEC && left >= 8) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(c) / 16; i++)
+            reinterpret_cast<uint4 *>(p)[i] = reinterpret_cast<const uint4 *>(&c)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i < left) p[i] = c.v[i];
+    }
+}
+
+// two fp32 -> two e4m3 (nearest, ties to even, saturating; NaN stays NaN), the first in the low byte
+__device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// s = max(max |v|, 2^-100) / 448 over the 16 lanes of a block (every lane of the warp calls it), q = e4m3(v / s) of this
+// lane's 8. v / s is taken as v * (1 / s), both correctly rounded: within 2^-23 of the quotient, so a value whose quotient
+// lies that near a border of two e4m3 values may fall to the other side. fmaxf drops NaN, so the others keep a scale;
+// an infinity makes s infinite and 1 / s zero: its own place becomes NaN and the block reads as NaN.
+__device__ __forceinline__ uint2 quantize_chunk(const float (&v)[8], float &s) {
+    float a = kAmaxFloor;
+#pragma unroll
+    for (int i = 0; i < 8; i++) a = fmaxf(a, fabsf(v[i]));
+#pragma unroll
+    for (int d = 8; d; d >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, d));
+    s = __fdiv_rn(a, kE4m3Max);
+    const float inv = __frcp_rn(s);
+    uint2 q;
+    q.x = cvt_e4m3x2(v[0] * inv, v[1] * inv) | cvt_e4m3x2(v[2] * inv, v[3] * inv) << 16;
+    q.y = cvt_e4m3x2(v[4] * inv, v[5] * inv) | cvt_e4m3x2(v[6] * inv, v[7] * inv) << 16;
+    return q;
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store_q(uint8_t *p, int left, uint2 q) {
+    if (VEC && left >= 8) {
+        *reinterpret_cast<uint2 *>(p) = q;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i < left) p[i] = (uint8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
+    }
+}
+
+}  // namespace inzg

@@ -10,8 +10,8 @@ import ctypes
 
 import numpy as np
 
-from ._lib import (DUMP_ROUTE, EP_HANDLE_BYTES, GEMM_SIMT, IO_DEVICE, N_STAGES, NO_FUSED, NO_GRAPH, PROFILE, Config, InzgError, MoeOpts, Stats, T_Q4L,
-                   T_Q8G, lib)
+from ._lib import (DUMP_ROUTE, EP_HANDLE_BYTES, GEMM_SIMT, IO_DEVICE, N_STAGES, NO_FUSED, NO_GRAPH, PROFILE, Config, GroupedMatmulArgs,
+                   InzgError, MatmulQ8Args, MoeOpts, RmsnormQ8Args, SiluMulQ8Args, Stats, T_Q4L, T_Q8G, lib)
 
 
 HC_RANK = 320  # INZG_HC_RANK: the hyper-connection bottleneck (src/model.h:14)
@@ -135,6 +135,56 @@ class MoePool:
     def shared_device(self, layer, n, x_ptr, y_ptr, n_batch, stream=None):
         self._check(lib.inzg_shared_expert(self._ctx, layer, n, ctypes.c_void_p(x_ptr), ctypes.c_void_p(y_ptr), n_batch,
                                            stream and ctypes.c_void_p(stream)), "shared_expert")
+
+    # -- experts in 8-bit floating point or bf16 / f16 (include/inzg.h): device pointers as ints, pitches in elements
+    # (0 = contiguous rows), types T_F32 / T_F16 / T_BF16 / T_E4M3; stream-ordered, no synchronisation. They use the
+    # pool's device, stream and error word (device_status), not its configured sizes. --
+    def rmsnorm_q8_device(self, n, cols, type, x_ptr, w_ptr, eps, ldx=0, res_ptr=None, ldres=0, sum_ptr=None, ldsum=0,
+                          y_ptr=None, ldy=0, q_ptr=None, ldq=0, s_ptr=None, lds=0, stream=None):
+        """h = x + res; sum = h; v = h / sqrt(mean(h^2) + eps) * w; y = v; q, s = v in e4m3 with a scale per 128 columns.
+        Each output is optional."""
+        a = RmsnormQ8Args(n, cols, type, x_ptr, ldx, res_ptr, ldres, sum_ptr, ldsum, w_ptr, eps, y_ptr, ldy, q_ptr, ldq,
+                          s_ptr, lds, stream)
+        st = lib.inzg_rmsnorm_q8(self._ctx, a)
+        if st:
+            self._check(st, "rmsnorm_q8")
+
+    def silu_mul_q8_device(self, n, cols, type, x_ptr, ldx=0, y_ptr=None, ldy=0, q_ptr=None, ldq=0, s_ptr=None, lds=0,
+                           stream=None):
+        """v = silu(x[:, :cols]) * x[:, cols:2 cols]; y = v; q, s = v in e4m3 with a scale per 128 columns."""
+        a = SiluMulQ8Args(n, cols, type, x_ptr, ldx, y_ptr, ldy, q_ptr, ldq, s_ptr, lds, stream)
+        st = lib.inzg_silu_mul_q8(self._ctx, a)
+        if st:
+            self._check(st, "silu_mul_q8")
+
+    def expert_lists_device(self, n, topk, n_expert, sel_ptr, off_ptr, rows_ptr, slots_ptr, w_ptr=None, w_out_ptr=None,
+                            stream=None):
+        """The selections sel [n][topk] in order of expert: off [n_expert + 1], token rows, slots t * topk + k, weights."""
+        st = lib.inzg_expert_lists(self._ctx, n, topk, n_expert, sel_ptr, w_ptr, off_ptr, rows_ptr, slots_ptr, w_out_ptr,
+                                   stream)
+        if st:
+            self._check(st, "expert_lists")
+
+    def matmul_q8_device(self, m, n, k, a_ptr, a_scale_ptr, w_ptr, w_scale_ptr, out_ptr, out_type, lda=0, lda_scale=0,
+                         ldw=0, ldo=0, stream=None):
+        """out [m][n] = a [m][k] w [n][k]^T, both e4m3 with block scales."""
+        a = MatmulQ8Args(m, n, k, a_ptr, lda, a_scale_ptr, lda_scale, w_ptr, ldw, w_scale_ptr, out_ptr, ldo, out_type,
+                         stream)
+        st = lib.inzg_matmul_q8(self._ctx, a)
+        if st:
+            self._check(st, "matmul_q8")
+
+    def grouped_matmul_device(self, type, groups, n, k, a_rows, entries, a_ptr, w_ptr, off_ptr, out_ptr, out_type, lda=0,
+                              ldw=0, ldo=0, a_scale_ptr=None, lda_scale=0, w_scale_ptr=None, in_rows_ptr=None,
+                              out_rows_ptr=None, out_scale_ptr=None, out_rows_n=None, stream=None):
+        """Entry i of group g (off [groups + 1]): out[out_rows[i]] = out_scale[i] * a[in_rows[i]] w[g]^T; w [groups][n][k].
+        out_rows_n: rows of out (default: entries)."""
+        a = GroupedMatmulArgs(type, groups, n, k, a_rows, entries, entries if out_rows_n is None else out_rows_n, a_ptr,
+                              lda, a_scale_ptr, lda_scale, w_ptr, ldw, w_scale_ptr, off_ptr, in_rows_ptr, out_rows_ptr,
+                              out_scale_ptr, out_ptr, ldo, out_type, stream)
+        st = lib.inzg_grouped_matmul(self._ctx, a)
+        if st:
+            self._check(st, "grouped_matmul")
 
     # expert parallelism with the exchange in the library (peer memory; include/inzg.h inzg_ep_*)
     def ep_attach(self, rank, world, capacity):
