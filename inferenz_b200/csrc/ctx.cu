@@ -308,6 +308,10 @@ inzg_ctx *inzg_create(const inzg_config *cfg, inzg_status *status) {
     c->fused_cnt = dalloc<int32_t>(fused_counter_ints((int)E, 8, (int)H), ok);
     if (ok && cudaMemset(c->fused_cnt, 0, sizeof(int32_t) * fused_counter_ints((int)E, 8, (int)H)) != cudaSuccess)
         ok = false;
+    // status words start clear: a call whose logits are given runs no router that would clear them
+    if (ok && (cudaMemset(c->meta, 0, sizeof(int32_t) * 16) != cudaSuccess ||
+               cudaMemset(c->sh_meta, 0, sizeof(int32_t) * 16) != cudaSuccess))
+        ok = false;
     c->op_err = dalloc<int32_t>(1, ok);
     if (ok && cudaMemset(c->op_err, 0, sizeof(int32_t)) != cudaSuccess) ok = false;
     if (!ok) {
