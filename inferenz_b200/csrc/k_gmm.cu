@@ -14,9 +14,10 @@
 //   warp 0      TMA producer: per 128-byte step of k a box of 128 weight rows and, unless they are gathered, the entries'
 //               rows in boxes of 16 or TN rows, 128-byte swizzle
 //   warp 1      allocates all 512 TMEM columns (4 accumulators per team), one lane issues 4 MMAs per stage
-//   warps 2-3   the entries' rows by index
-//   warps 4-11  fold and write, thread = a row of w. TN = 128: all eight warps share an item, every other 32 entries;
-//               TN = 32: the two warpgroups take the items in turn, so one writes while the other folds
+//   warps 2-3   stage as * ws and where each entry's result goes, ahead of the fold
+//   warps 4-7   the entries' rows by index
+//   warps 8-15  fold and write, thread = a row of w. TN = 128 (bf16 / f16): all eight warps share an item, every other 32
+//               entries; TN = 32: the two warpgroups take the items in turn, so one writes while the other folds
 // Persistent: one CTA per SM walks the items; the offsets are turned into tile numbers by every CTA for itself, which
 // costs a read of off and a scan instead of a launch. Every mbarrier wait is bounded; on expiry the CTA records an
 // error, drains what it issued, frees its TMEM and returns.
@@ -29,24 +30,18 @@
 
 namespace inzg {
 
-constexpr int GM = 128;      // weight rows of an item
-constexpr int kGmmKc = 8;    // k blocks whose scales are staged at once
+constexpr int kGmmThreads = 512;  // sixteen warps, as above
+constexpr int kGmmGatherWarps = 4;
+constexpr int GM = 128;    // weight rows of an item
+constexpr int kGmmKc = 8;  // k blocks whose scales are staged at once
 
 template <int TN>
 struct GmmCfg {
-    static constexpr int kTeams = TN <= 32 ? 2 : 1, kTeamWarps = 8 / kTeams, kTeamThreads = kTeamWarps * 32;
+    static constexpr int kTeams = TN <= 32 ? 2 : 1, kTeamWarps = 8 / kTeams;
     static constexpr int kStages = TN <= 32 ? 10 : 6, kStage = (GM + TN) * kGmmBytes;
     static constexpr int kAcc = 4;                              // accumulators of TN columns, per team: a team waits for its
                                                                 // own alone, so it is never two phases of one ahead
     static constexpr int kChunks = TN / 32 / (2 / kTeams);      // 32-entry chunks per thread
-    static constexpr int kPre = kGmmKc * TN / kTeamThreads;     // staged scales per thread
-    static constexpr int kParts = kGmmKc / kPre;                // threads per entry in the staging
-};
-
-// where an entry's result goes: its row of out (null: not written) and its weight
-struct alignas(16) GmmTo {
-    char *row;
-    float w;
 };
 
 template <int TN>
@@ -55,8 +50,7 @@ struct GmmShared {
     uint64_t full[C::kStages], empty[C::kStages], acc_full[C::kTeams][C::kAcc], acc_empty[C::kTeams][C::kAcc], drain;
     uint32_t tmem_base;
     int abort, never;
-    alignas(16) float p[C::kTeams][2][kGmmKc][TN];  // as * ws of the staged blocks
-    GmmTo to[C::kTeams][2][TN];
+    GmmStaged<TN, C::kTeams, 1, kGmmKc> staged;
     GmmWalk walk;
 };
 
@@ -64,7 +58,7 @@ template <class T>
 __device__ __forceinline__ void gmm_put(const GmmTo &t, int64_t col, float v) {
     T o;
     from_f32(v * t.w, o);
-    if (t.row) reinterpret_cast<T *>(t.row)[col] = o;
+    if (t.row) store_global(reinterpret_cast<T *>(t.row) + col, o);
 }
 
 // map_w: [groups * n][k] in 128-row boxes; map_a16 / map_a: the rows of a in boxes of 16 / TN rows
@@ -75,7 +69,8 @@ gmm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
     using C = GmmCfg<TN>;
     constexpr int ST = C::kStages, NA = C::kAcc;
     extern __shared__ __align__(1024) uint8_t gmm_dyn[];
-    uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(gmm_dyn) + 1023) & ~uintptr_t(1023));
+    // an offset, not a rounded address: the compiler has to see shared memory, or every access becomes a generic one
+    uint8_t *ring = gmm_dyn + (-smem_u32(gmm_dyn) & 1023u);
     GmmShared<TN> &S = *reinterpret_cast<GmmShared<TN> *>(ring + ST * C::kStage);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int *abort = &S.abort;
@@ -93,6 +88,7 @@ gmm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
                 mbar_init(&S.acc_empty[t][b], C::kTeamWarps);
             }
         mbar_init(&S.drain, 1);
+        gmm_staged_init(S.staged);
         S.abort = 0;
         S.never = 0;
         S.walk.bad = 0;
@@ -103,180 +99,158 @@ gmm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = S.tmem_base;
-    gmm_walk_init<TN>(S.walk, A);
-    const int nitems = S.walk.bad ? 0 : S.walk.tstart[A.groups] * A.nrb;
-    if (S.walk.bad && threadIdx.x == 0) atomicCAS(A.err, kErrNone, kErrOverflow);
+    const int nitems = gmm_walk_init<TN, kGmmThreads>(S.walk, A, blockIdx.x, gridDim.x);
     const int steps = A.steps;
 
-    if (warp == 0) {
-        // ---------------- TMA producer ----------------
-        int kg = 0;  // stages issued by this CTA
-        bool ok = true;
-        for (int item = blockIdx.x; item < nitems && ok; item += gridDim.x) {
-            const GmmItem I = gmm_item<TN>(S.walk, A.groups, A.nrb, item);
-            const int n16 = (I.nt + 15) & ~15;
-            const bool whole = I.nt > TN / 2;
-            const uint32_t bytes = (GM + (A.in_rows ? 0 : whole ? TN : n16)) * kGmmBytes;
-            for (int k = 0; k < steps; k++, kg++) {
-                const int s = kg % ST, x = k * (kGmmBytes / kElem);
-                if (kg >= ST) ok = mbar_wait(&S.empty[s], ((kg / ST) - 1) & 1, abort);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                uint8_t *stage = ring + s * C::kStage;
-                if (lane == 0) {
-                    mbar_expect_tx(&S.full[s], bytes);
-                    tma_load_2d(stage, &map_w, x, I.g * A.n + I.rb * GM, &S.full[s]);
-                    if (!A.in_rows && whole) tma_load_2d(stage + GM * kGmmBytes, &map_a, x, I.base, &S.full[s]);
-                }
-                __syncwarp();
-                if (!A.in_rows && !whole && lane * 16 < n16)
-                    tma_load_2d(stage + (GM + lane * 16) * kGmmBytes, &map_a16, x, I.base + lane * 16, &S.full[s]);
-            }
-        }
-        if (!ok) S.abort = 1;
-        // every issued copy has landed before the CTA may leave (bounded; each slot's latest phase)
-        for (int k = max(0, kg - ST); k < kg; k++) mbar_wait(&S.full[k % ST], (k / ST) & 1, never);
-    } else if (warp == 1) {
-        // ---------------- MMA issuer ----------------
-        if (lane == 0) {
-            bool ok = true;
-            int kg = 0, it = 0;  // stages consumed, items begun by this CTA
-            for (int item = blockIdx.x; item < nitems && ok; item += gridDim.x, it++) {
-                const int team = it % C::kTeams;
-                int bg = it / C::kTeams * (F8 ? steps : 1);  // accumulators handed to this team so far
-                const GmmItem I = gmm_item<TN>(S.walk, A.groups, A.nrb, item);
-                const uint32_t idesc = A.idesc | (uint32_t)(((I.nt + 15) & ~15) >> 3) << 17;
-                for (int k = 0; k < steps; k++, kg++) {
-                    const int s = kg % ST, buf = bg % NA;
-                    const bool open = F8 || k == 0, close = F8 || k == steps - 1;
-                    if (open && bg >= NA && !mbar_wait(&S.acc_empty[team][buf], ((bg / NA) - 1) & 1, abort)) { ok = false; break; }
-                    if (!mbar_wait(&S.full[s], (kg / ST) & 1, abort)) { ok = false; break; }
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint8_t *stage = ring + s * C::kStage;
-                    const uint64_t da = gmm_desc(stage), db = gmm_desc(stage + GM * kGmmBytes);
-#pragma unroll
-                    for (int j = 0; j < kGmmBytes / 32; j++)  // 32 bytes of k per MMA
-                        gmm_mma<F8>(tmem + (team * NA + buf) * TN, da + (uint64_t)(j * 2), db + (uint64_t)(j * 2), idesc, !(open && j == 0));
-                    gmm_commit(&S.empty[s]);
-                    if (close) {
-                        gmm_commit(&S.acc_full[team][buf]);
-                        bg++;
+    // registers: 128 per thread at launch, 16 warps; 8 * 88 + 8 * 168 = 16 * 128
+    if (warp < 8) {
+        if (TN > 32) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 0) {
+            // ---------------- TMA producer ----------------
+            if (gmm_elect()) {
+                int issued = 0;  // stages, counted up to the ring's size
+                bool ok = true;
+                GmmSlot<ST> slot;
+                for (int item = blockIdx.x, n = 0; item < nitems && ok; item += gridDim.x, n++) {
+                    const GmmItem I = gmm_item<TN>(S.walk, A, item, n);
+                    const bool whole = I.nt > 16;
+                    const uint32_t bytes = (GM + (A.in_rows ? 0 : whole ? TN : 16)) * kGmmBytes;
+                    const int wrow = I.g * A.n + I.rb * GM;
+                    for (int k = 0, x = 0; k < steps; k++, x += kGmmBytes / kElem) {
+                        if (issued == ST) {
+                            if (!(ok = mbar_wait(&S.empty[slot.i], slot.parity ^ 1, abort))) break;
+                        } else {
+                            issued++;
+                        }
+                        uint8_t *stage = ring + slot.i * C::kStage;
+                        uint64_t *full = &S.full[slot.i];
+                        mbar_expect_tx(full, bytes);
+                        tma_load_2d(stage, &map_w, x, wrow, full);
+                        if (!A.in_rows) {
+                            if (whole) tma_load_2d(stage + GM * kGmmBytes, &map_a, x, I.base, full);
+                            else tma_load_2d(stage + GM * kGmmBytes, &map_a16, x, I.base, full);
+                        }
+                        slot.next();
                     }
                 }
+                if (!ok) S.abort = 1;
+                // every issued copy has landed before the CTA may leave (bounded): the last round of each slot in use
+                for (int k = 0; k < issued; k++) {
+                    if (issued == ST) mbar_wait(&S.full[slot.i], slot.parity ^ 1, never);
+                    else mbar_wait(&S.full[k], 0, never);
+                    slot.next();
+                }
             }
-            if (!ok) S.abort = 1;
-            // every MMA issued by this CTA has completed before TMEM and shared memory are released (bounded)
-            gmm_commit(&S.drain);
-            mbar_wait(&S.drain, 0, never);
+            __syncwarp();
+        } else if (warp == 1) {
+            // ---------------- MMA issuer ----------------
+            if (gmm_elect()) {
+                bool ok = true;
+                GmmSlot<ST> slot;
+                struct Accs {  // one team's accumulators
+                    GmmSlot<NA> at;
+                    int given = 0;  // handed over, counted up to NA
+                };
+                Accs mine, other;  // of the current item's team and (two teams) of the next item's: they change places
+                const uint64_t desc0 = gmm_desc(ring);
+                for (int item = blockIdx.x, team = 0, n = 0; item < nitems && ok; item += gridDim.x, team = (team + 1) % C::kTeams, n++) {
+                    const GmmItem I = gmm_item<TN>(S.walk, A, item, n);
+                    const uint32_t idesc = A.idesc | (uint32_t)(((I.nt + 15) & ~15) >> 3) << 17;
+                    for (int k = 0; k < steps; k++) {
+                        const bool open = F8 || k == 0, close = F8 || k == steps - 1;
+                        if (open) {
+                            if (mine.given == NA) ok = mbar_wait(&S.acc_empty[team][mine.at.i], mine.at.parity ^ 1, abort);
+                            else mine.given++;
+                        }
+                        if (!ok || !(ok = mbar_wait(&S.full[slot.i], slot.parity, abort))) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint64_t da = desc0 + (uint64_t)(slot.i * (C::kStage >> 4));
+                        gmm_mma_stage<F8>(tmem + (team * NA + mine.at.i) * TN, da, da + (GM * kGmmBytes >> 4), idesc, open);
+                        gmm_commit(&S.empty[slot.i]);
+                        if (close) {
+                            gmm_commit(&S.acc_full[team][mine.at.i]);
+                            mine.at.next();
+                        }
+                        slot.next();
+                    }
+                    if constexpr (C::kTeams == 2) {
+                        const Accs t = mine;
+                        mine = other;
+                        other = t;
+                    }
+                }
+                if (!ok) S.abort = 1;
+                // every MMA issued by this CTA has completed before TMEM and shared memory are released (bounded)
+                gmm_commit(&S.drain);
+                mbar_wait(&S.drain, 0, never);
+            }
+            __syncwarp();
+        } else if (warp < 4) {
+            if (!gmm_stage_walk<F8, TN>(S.staged, S.walk, A, nitems, abort)) S.abort = 1;
+        } else if (warp >= 4) {
+            if (A.in_rows && !gmm_gather<TN, ST, kGmmGatherWarps>(S.walk, A, threadIdx.x - 128, nitems, ring, C::kStage, GM * kGmmBytes,
+                                                                  S.full, S.empty, abort))
+                S.abort = 1;
         }
-        __syncwarp();
-    } else if (warp < 4) {
-        if (A.in_rows && !gmm_gather<TN, ST>(S.walk, A, nitems, ring, C::kStage, GM * kGmmBytes, S.full, S.empty, abort))
-            S.abort = 1;
     } else {
         // ---------------- fold and write ----------------
-        // TMEM lane quadrant = warp % 4. One team: warps 4-7 take the even 32-entry chunks of every item, warps 8-11 the
+        if (TN > 32) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        // TMEM lane quadrant = warp % 4. One team: warps 8-11 take the even 32-entry chunks of every item, warps 12-15 the
         // odd ones; two teams: each takes every other item whole.
-        const int sub = warp & 3, upper = (warp - 4) >> 2;
+        const int sub = warp & 3, upper = (warp - 8) >> 2;
         const int team = C::kTeams == 2 ? upper : 0, c_first = C::kTeams == 2 ? 0 : upper, c_step = C::kTeams == 2 ? 1 : 2;
-        const int et = (threadIdx.x - 128) % C::kTeamThreads;
-        const int esize = A.out_type == INZG_T_F32 ? 4 : 2;
-        bool ok = true;  // a thread whose wait ran out goes on without waiting or writing: the team's barriers stay matched
-        const int nkc = F8 ? (steps + kGmmKc - 1) / kGmmKc : 1, accs = F8 ? steps : 1;
-        const int pe = et / C::kParts, pk = (et % C::kParts) * C::kPre;  // staging: entry, first of its blocks
-        float pre[C::kPre];
-        // what the next item needs is loaded while the current one folds: the rows behind its entries first, the scales of its
-        // first blocks once those are there
-        int row = 0;
-        GmmTo to{nullptr, 0.0f};
-        bool bad_row = false;
-        auto load_entry = [&](const GmmItem &I) {
-            if (F8) {
-                const int i = I.base + min(pe, I.nt - 1);
-                const int v = A.in_rows ? A.in_rows[i] : i;
-                row = (unsigned)v < (unsigned)A.a_rows ? v : 0;
-            }
-            to.row = nullptr;
-            if (et < I.nt) {
-                const int i = I.base + et;
-                const int o = A.out_rows ? A.out_rows[i] : i;
-                bad_row = (unsigned)o >= (unsigned)A.out_rows_n || (A.in_rows && (unsigned)A.in_rows[i] >= (unsigned)A.a_rows);
-                if (!bad_row) to.row = static_cast<char *>(A.out) + (int64_t)o * A.ldo * esize;
-                to.w = A.out_scale ? A.out_scale[i] : 1.0f;
-            }
-        };
-        auto load_scales = [&](const GmmItem &I, int kc) {
-            const float *as = A.as + (int64_t)row * A.ldas;
-            const float *ws = A.ws + ((int64_t)I.g * A.nrb128 + I.rb) * steps;
-#pragma unroll
-            for (int j = 0; j < C::kPre; j++) {
-                const int b = kc * kGmmKc + pk + j;
-                pre[j] = b < steps && pe < I.nt ? __ldg(as + b) * __ldg(ws + b) : 0.0f;
-            }
-        };
-        const int first = blockIdx.x + team * gridDim.x, stride = C::kTeams * gridDim.x;
-        GmmItem I{0, 0, 0, 0}, N{0, 0, 0, 0};
-        if (first < nitems) {
-            N = gmm_item<TN>(S.walk, A.groups, A.nrb, first);
-            load_entry(N);
-            if (F8) load_scales(N, 0);
-        }
-        int it = 0, cbuf = 0;  // items of this team, chunks of scales staged so far
-        for (int item = first; item < nitems; item += stride, it++) {
-            I = N;
-            const bool more = item + stride < nitems;
-            GmmTo(&tos)[TN] = S.to[team][it & 1];
-            if (et < TN) tos[et] = to;
-            if (bad_row) atomicCAS(A.err, kErrNone, kErrBadSlot);
-            bad_row = false;
-            const int bg0 = it * accs;  // accumulators of this team before this item
+        bool ok = true;
+        GmmSlot<NA> acc;
+        GmmSlot<kGmmRing> ps, ts;
+        const uint32_t lanes = tmem + ((uint32_t)(sub * 32) << 16) + team * NA * TN + c_first * 32;
+        for (int item = blockIdx.x + team * gridDim.x, n = team; item < nitems && ok; item += C::kTeams * gridDim.x, n += C::kTeams) {
+            const GmmItem I = gmm_item<TN>(S.walk, A, item, n);
             float2 f[C::kChunks * 16];
 #pragma unroll
             for (int j = 0; j < C::kChunks * 16; j++) f[j] = make_float2(0.0f, 0.0f);
-            for (int kc = 0; kc < nkc; kc++, cbuf++) {
-                float(&p)[kGmmKc][TN] = S.p[team][cbuf & 1];
-                if (F8)
-#pragma unroll
-                    for (int j = 0; j < C::kPre; j++) p[pk + j][pe] = pre[j];
-                asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(C::kTeamThreads) : "memory");
-                if (F8 && kc + 1 < nkc) load_scales(I, kc + 1);
-                if (more && kc + 1 == nkc) {  // before that `row` still serves this item's later chunks
-                    N = gmm_item<TN>(S.walk, A.groups, A.nrb, item + stride);
-                    load_entry(N);
-                }
-                const int nb = F8 ? min(kGmmKc, steps - kc * kGmmKc) : 1;
+            for (int b0 = 0; b0 < (F8 ? steps : 1); b0 += kGmmKc) {
+                if (F8) ok = mbar_wait(&S.staged.p_full[team][ps.i], ps.parity, abort);
+                const float(&p)[kGmmKc][TN] = S.staged.p[team][ps.i][0];
+                const int nb = F8 ? min(kGmmKc, steps - b0) : 1;
                 for (int b = 0; b < nb; b++) {
-                    const int bg = bg0 + kc * kGmmKc + b, buf = bg % NA;
-                    if (ok && !mbar_wait(&S.acc_full[team][buf], (bg / NA) & 1, abort)) ok = false;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (ok) ok = mbar_wait(&S.acc_full[team][acc.i], acc.parity, abort);
                     ok = __all_sync(0xffffffffu, ok);
-                    if (ok) {
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-                        for (int c = 0; c < C::kChunks; c++) {
-                            const int c0 = (c_first + c_step * c) * 32;
-                            if (c0 >= I.nt) continue;
-                            float v[32];
-                            gmm_ld32(tmem + ((uint32_t)(sub * 32) << 16) + (team * NA + buf) * TN + c0, v);
+                    for (int c = 0; c < C::kChunks; c++) {
+                        const int c0 = (c_first + c_step * c) * 32;
+                        if (c0 >= I.nt) continue;
+                        float v[32];
+                        gmm_ld32(lanes + acc.i * TN + c_step * c * 32, v);
 #pragma unroll
-                            for (int j = 0; j < 8; j++) {
-                                const int o = c * 16 + j * 2;
-                                if (F8) {
-                                    const float4 s4 = *reinterpret_cast<const float4 *>(&p[b][c0 + j * 4]);
-                                    f[o] = __ffma2_rn(make_float2(v[j * 4], v[j * 4 + 1]), make_float2(s4.x, s4.y), f[o]);
-                                    f[o + 1] = __ffma2_rn(make_float2(v[j * 4 + 2], v[j * 4 + 3]), make_float2(s4.z, s4.w), f[o + 1]);
-                                } else {
-                                    f[o] = make_float2(v[j * 4], v[j * 4 + 1]);
-                                    f[o + 1] = make_float2(v[j * 4 + 2], v[j * 4 + 3]);
-                                }
+                        for (int j = 0; j < 8; j++) {
+                            const int o = c * 16 + j * 2;
+                            if (F8) {
+                                const float4 s4 = *reinterpret_cast<const float4 *>(&p[b][c0 + j * 4]);
+                                f[o] = __ffma2_rn(make_float2(v[j * 4], v[j * 4 + 1]), make_float2(s4.x, s4.y), f[o]);
+                                f[o + 1] = __ffma2_rn(make_float2(v[j * 4 + 2], v[j * 4 + 3]), make_float2(s4.z, s4.w), f[o + 1]);
+                            } else {
+                                f[o] = make_float2(v[j * 4], v[j * 4 + 1]);
+                                f[o + 1] = make_float2(v[j * 4 + 2], v[j * 4 + 3]);
                             }
                         }
                     }
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&S.acc_empty[team][buf]);
+                    if (lane == 0) mbar_arrive(&S.acc_empty[team][acc.i]);
+                    acc.next();
                 }
-                if (F8 && more && kc + 1 == nkc) load_scales(N, 0);
+                if (!ok) break;
+                if (F8) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&S.staged.p_empty[team][ps.i]);
+                    ps.next();
+                }
             }
+            if (ok) ok = mbar_wait(&S.staged.to_full[team][ts.i], ts.parity, abort);
+            ok = __all_sync(0xffffffffu, ok);
+            const GmmTo(&tos)[TN] = S.staged.to[team][ts.i];
             const int col = I.rb * GM + sub * 32 + lane;
             if (ok && col < A.n) {
                 auto write = [&](auto zero) {
@@ -285,6 +259,7 @@ gmm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
                     for (int j8 = 0; j8 < C::kChunks * 4; j8++) {
                         const int t = (c_first + c_step * (j8 >> 2)) * 32 + (j8 & 3) * 8;
                         if (t >= I.nt) continue;
+                        asm volatile("" ::: "memory");  // eight targets at a time, or they take the registers of all
 #pragma unroll
                         for (int j = 0; j < 8; j++) gmm_put<T>(tos[t + j], col, (j & 1) ? f[j8 * 4 + (j >> 1)].y : f[j8 * 4 + (j >> 1)].x);
                     }
@@ -293,6 +268,9 @@ gmm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
                 else if (A.out_type == INZG_T_BF16) write(__nv_bfloat16());
                 else write(__half());
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&S.staged.to_empty[team][ts.i]);
+            ts.next();
         }
         if (!ok) S.abort = 1;
     }
@@ -332,15 +310,13 @@ static_assert(gmm_smem<32>() <= 227 * 1024 && gmm_smem<128>() <= 227 * 1024, "sh
 void gmm_set_attributes() {
     cudaFuncSetAttribute(gmm_kernel<true, 32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)gmm_smem<32>());
     cudaFuncSetAttribute(gmm_kernel<false, 32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)gmm_smem<32>());
-    cudaFuncSetAttribute(gmm_kernel<true, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)gmm_smem<128>());
     cudaFuncSetAttribute(gmm_kernel<false, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)gmm_smem<128>());
     gmm_large_set_attributes();
 }
 
-template <int TN>
+template <bool F8, int TN>
 static int gmm_launch(const inzg_grouped_matmul_args &G, const GmmArgs &A, int num_sms, cudaStream_t st) {
-    const bool f8 = G.type == INZG_T_E4M3;
-    const int elem = f8 ? 1 : 2;
+    constexpr int elem = F8 ? 1 : 2;
     const int64_t lda = G.lda ? G.lda : G.k, ldw = G.ldw ? G.ldw : G.k;
     CUtensorMap map_w, map_a16, map_a;
     if (!gmm_map(&map_w, G.w, elem, (int64_t)G.groups * G.n, G.k, ldw, GM) ||
@@ -348,14 +324,9 @@ static int gmm_launch(const inzg_grouped_matmul_args &G, const GmmArgs &A, int n
         return -1;
     const int64_t tiles = std::min<int64_t>(G.entries, G.entries / TN + G.groups);  // at most so many
     const int grid = (int)std::min<int64_t>(num_sms, tiles * A.nrb);
-    if (f8) gmm_kernel<true, TN><<<grid, kGmmThreads, gmm_smem<TN>(), st>>>(map_w, map_a16, map_a, A);
-    else gmm_kernel<false, TN><<<grid, kGmmThreads, gmm_smem<TN>(), st>>>(map_w, map_a16, map_a, A);
+    gmm_kernel<F8, TN><<<grid, kGmmThreads, gmm_smem<TN>(), st>>>(map_w, map_a16, map_a, A);
     return 1;
 }
-
-// Many entries per group: the product is bound by the tensor pipe and the fold, and the kernel with 128 x 256 tiles is
-// the faster one.
-static bool gmm_use_large(const inzg_grouped_matmul_args &G) { return G.entries >= 256 * (int64_t)G.groups; }
 
 int launch_grouped_matmul(const inzg_grouped_matmul_args &G, int num_sms, int32_t *err, cudaStream_t st) {
     const int elem = G.type == INZG_T_E4M3 ? 1 : 2;
@@ -384,9 +355,18 @@ int launch_grouped_matmul(const inzg_grouped_matmul_args &G, int num_sms, int32_
     // fp32 accumulators; e4m3 (0), bf16 (1) or f16 (0) operands, both K-major; M = 128
     const uint32_t fmt = G.type == INZG_T_BF16 ? 1u : 0u;
     A.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(GM >> 4) << 24);
-    if (gmm_use_large(G)) return gmm_large_launch(G, A, num_sms, st);
-    if (G.entries <= 16 * (int64_t)G.groups) return gmm_launch<32>(G, A, num_sms, st);
-    return gmm_launch<128>(G, A, num_sms, st);
+    // Which kernel, by the entries per group (measured at k = 2048 and 2560 with 1280 columns, us):
+    //   bf16, 64 groups:    20 a group: 32-entry tiles 76, 128-entry tiles 81; 30 a group: 88, 81; 160 a group: 265, 121
+    //   e4m3, 64 groups:    40 a group: 32-entry tiles 47, 128 x 256 tiles 53; 62 a group: 61, 53; 160 a group: 124, 67
+    //   e4m3, 8 groups:     64 a group: 32-entry tiles 15, 128 x 256 tiles 20; 128 a group: 21, 20
+    // The last case has fewer large tiles than half the SMs, and small ones fill the GPU better.
+    if (G.type != INZG_T_E4M3) {
+        if (G.entries <= 24 * (int64_t)G.groups) return gmm_launch<false, 32>(G, A, num_sms, st);
+        return gmm_launch<false, 128>(G, A, num_sms, st);
+    }
+    const int64_t large_items = std::min<int64_t>(G.entries, G.entries / 128 + G.groups) * ((G.n + 255) / 256);
+    if (G.entries <= (large_items <= num_sms / 2 ? 96 : 48) * (int64_t)G.groups) return gmm_launch<true, 32>(G, A, num_sms, st);
+    return gmm_large_launch(G, A, num_sms, st);
 }
 
 }  // namespace inzg

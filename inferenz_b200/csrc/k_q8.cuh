@@ -20,6 +20,19 @@ __device__ __forceinline__ void from_f32(float v, float &o) { o = v; }
 __device__ __forceinline__ void from_f32(float v, __half &o) { o = __float2half_rn(v); }
 __device__ __forceinline__ void from_f32(float v, __nv_bfloat16 &o) { o = __float2bfloat16_rn(v); }
 
+// plain stores that are said to be to global memory (a pointer that passed through shared memory is not known to be); under an
+// `if` they become predicated instructions
+__device__ __forceinline__ void store_global(float *p, float v) { asm volatile("st.global.f32 [%0], %1;" ::"l"(p), "f"(v) : "memory"); }
+__device__ __forceinline__ void store_global(__half *p, __half v) {
+    asm volatile("st.global.b16 [%0], %1;" ::"l"(p), "h"(__half_as_ushort(v)) : "memory");
+}
+__device__ __forceinline__ void store_global(__nv_bfloat16 *p, __nv_bfloat16 v) {
+    asm volatile("st.global.b16 [%0], %1;" ::"l"(p), "h"(__bfloat16_as_ushort(v)) : "memory");
+}
+__device__ __forceinline__ void store_global(uint4 *p, uint4 v) {
+    asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
 // A thread's chunk: 8 neighbouring elements (16 or 32 bytes), so that a block of 128 columns is 16 lanes of one warp.
 template <class T>
 struct alignas(16) Chunk {
