@@ -325,6 +325,7 @@ inzg_ctx *inzg_create(const inzg_config *cfg, inzg_status *status) {
     gemv_set_attributes();
     gemm_tc_set_attributes();
     gmm_set_attributes();
+    lists_set_attributes();
     c->have_tc = make_tma_map_i8(c->map_xqe.bytes, c->xqe, NE, H, 128) && make_tma_map_i8(c->map_dq.bytes, c->dq256, NE, FF, 128);
     for (int i = 0; i <= INZG_N_STAGES; i++) cudaEventCreate(&c->ev[i]);
     cudaStreamCreateWithFlags(&c->capture_stream, cudaStreamNonBlocking);

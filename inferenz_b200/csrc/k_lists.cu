@@ -1,103 +1,170 @@
-// k_lists.cu -- the entries of the router's selections in order of expert, on sm_100a (inzg_expert_lists).
+// k_lists.cu -- the entries of the router's selections in order of expert, on sm_100a (inzg_expert_lists): a stable counting sort
+// without scratch in global memory; its shared-memory atomics only count and set bits, so the order is fixed.
 //
-// One block per expert, no scratch and no atomics: the block reads every selection, counts those of smaller experts (its
-// list's offset) and its own, and writes its own in slot order. A warp owns a contiguous run of the entries, so an
-// entry's place is off + (own entries of earlier warps) + (own entries of this warp so far) + its rank in the warp's
-// ballot: the order is fixed. Work is n_expert * n * topk compares, each entry read by every block from L2.
+// One block, or for more than 2048 entries a cluster of eight. A warp owns a contiguous run of the entries, a row of
+// counters in shared memory, one per expert, and a row of lane masks: within a step of 32 entries the lanes set their bits in
+// their experts' masks (match.any, which does the same, goes through the distinct values one by one and was slower), so that
+//   place = (entries of smaller experts) + (own expert: earlier blocks, earlier warps, earlier steps, lower lanes)
+// The blocks of the cluster read one another's totals through distributed shared memory. Each entry is read twice; what bounds it
+// is the chain of two passes, a scan over the experts and two cluster barriers. A block per expert (or per four) that counted
+// every entry for itself took 20 to 26 us at 4096 tokens, top-10.
 #include <algorithm>
 
 #include "inzg_internal.h"
+#include "k_async.cuh"
 #include "k_launch.h"
 
 namespace inzg {
 
-constexpr int kListWarps = 16;
+constexpr int kListThreads = 1024, kListCluster = 8, kListCounters = 24576;  // counters of all warps, and as many masks: 192 KB
 
-template <bool VEC>
-__global__ void __launch_bounds__(kListWarps * 32) expert_lists_kernel(const int32_t *__restrict__ sel, const float *__restrict__ w,
-                                                                       int entries, int topk, int E, int32_t *__restrict__ off,
-                                                                       int32_t *__restrict__ rows, int32_t *__restrict__ slots,
-                                                                       float *__restrict__ w_out, int32_t *err) {
-    __shared__ int s_less[kListWarps], s_own[kListWarps];
-    const int e = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
-    // whole 128-entry steps per warp
-    const int steps = (entries + nw * 128 - 1) / (nw * 128);
-    const int first = warp * steps * 128;
-    auto load = [&](int i) {  // entries i .. i + 3; -1 behind the last
-        int4 v = make_int4(-1, -1, -1, -1);
-        if (VEC && i + 3 < entries) {
-            v = *reinterpret_cast<const int4 *>(sel + i);
-        } else {
-            if (i < entries) v.x = sel[i];
-            if (i + 1 < entries) v.y = sel[i + 1];
-            if (i + 2 < entries) v.z = sel[i + 2];
-            if (i + 3 < entries) v.w = sel[i + 3];
-        }
-        return v;
-    };
-    int less = 0, own = 0;
+__device__ __forceinline__ void lists_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int lists_remote(const int *p, int rank) {  // *p of block `rank` of the cluster
+    uint32_t a;
+    int v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a));  // volatile: stays between the cluster's barriers
+    return v;
+}
+
+// shared: counters [warps][E], masks [warps][E], then this block's totals [E] and the first place of each expert's entries of this
+// block [E]
+template <int CLUSTER>
+__global__ void __launch_bounds__(kListThreads)
+expert_lists_kernel(const int32_t *__restrict__ sel, const float *__restrict__ w, int entries, int topk, int E, int32_t *__restrict__ off,
+                    int32_t *__restrict__ rows, int32_t *__restrict__ slots, float *__restrict__ w_out, int32_t *err) {
+    extern __shared__ __align__(16) int lists_dyn[];
+    __shared__ int s_scan[32];
+    const int nw = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = CLUSTER > 1 ? blockIdx.x : 0;
+    int *count = lists_dyn + warp * E, *total = lists_dyn + 2 * nw * E, *place = total + E;
+    uint32_t *mask = reinterpret_cast<uint32_t *>(count + nw * E);
+    const int steps = (int)(((int64_t)entries + CLUSTER * nw * 32 - 1) / (CLUSTER * nw * 32));
+    const int64_t first = (int64_t)(rank * nw + warp) * steps * 32 + lane;
+    int next = steps && first < entries ? sel[first] : -1;
+    for (int i = threadIdx.x; i < (2 * nw * E + 3) / 4; i += blockDim.x) reinterpret_cast<int4 *>(lists_dyn)[i] = make_int4(0, 0, 0, 0);
+    __syncthreads();
+    const uint32_t below = (1u << lane) - 1;
+    // first pass: entries per expert of this warp's run
     bool bad = false;
     for (int j = 0; j < steps; j++) {
-        const int i = first + j * 128 + lane * 4;
-        const int4 v = load(i);
-        const int a[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-            less += a[c] >= 0 && a[c] < e;
-            own += a[c] == e;
-            bad |= a[c] >= E;
-        }
+        const int e = next;
+        const int64_t i = first + (j + 1) * 32;
+        if (j + 1 < steps) next = i < entries ? sel[i] : -1;
+        bad |= e >= E;
+        if ((uint32_t)e < (uint32_t)E) atomicAdd(&count[e], 1);
     }
-    if (bad && e == 0) atomicCAS(err, kErrNone, kErrBadExpert);
-    less = __reduce_add_sync(0xffffffffu, less);
-    own = __reduce_add_sync(0xffffffffu, own);
-    if (lane == 0) {
-        s_less[warp] = less;
-        s_own[warp] = own;
-    }
+    if (bad) atomicCAS(err, kErrNone, kErrBadExpert);
     __syncthreads();
-    int base = 0, total = 0;
-    for (int k = 0; k < nw; k++) {
-        base += s_less[k] + (k < warp ? s_own[k] : 0);
-        total += s_less[k] + s_own[k];
+    // per expert: the warps' counts become what the warps before have; a thread has `per` neighbouring experts
+    const int per = (E + blockDim.x - 1) / blockDim.x, e0 = threadIdx.x * per, e1 = min(e0 + per, E);
+    for (int e = e0; e < e1; e++) {
+        int run = 0;
+        for (int k = 0; k < nw; k += 8) {  // eight loads at a time
+            int t[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) t[j] = k + j < nw ? lists_dyn[(k + j) * E + e] : 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                if (k + j < nw) lists_dyn[(k + j) * E + e] = run;
+                run += t[j];
+            }
+        }
+        total[e] = run;
     }
-    if (threadIdx.x == 0) {
-        off[e] = total - [&] { int t = 0; for (int k = 0; k < nw; k++) t += s_own[k]; return t; }();
-        if (e == E - 1) off[E] = total;
+    if (CLUSTER > 1) lists_cluster_sync();
+    // the cluster's entries per expert, and a scan over the experts
+    int mine = 0;
+    for (int e = e0; e < e1; e++) {
+        int before = 0, all = 0, t[CLUSTER];
+#pragma unroll
+        for (int q = 0; q < CLUSTER; q++) t[q] = CLUSTER > 1 ? lists_remote(total + e, q) : total[e];
+#pragma unroll
+        for (int q = 0; q < CLUSTER; q++) {
+            if (q < rank) before += t[q];
+            all += t[q];
+        }
+        place[e] = mine + before;  // within this thread's experts so far
+        if (rank == 0) off[e] = mine;
+        mine += all;
     }
-    if (own == 0) return;
+    int scan = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const int t = __shfl_up_sync(0xffffffffu, scan, d);
+        if (lane >= d) scan += t;
+    }
+    if (lane == 31) s_scan[warp] = scan;
+    __syncthreads();
+    int start = scan - mine;
+    for (int k = 0; k < warp; k++) start += s_scan[k];
+    for (int e = e0; e < e1; e++) {
+        place[e] += start;
+        if (rank == 0) off[e] += start;
+    }
+    if (rank == 0 && e0 < E && e1 == E) off[E] = start + mine;
+    __syncthreads();
+    // second pass: every entry to its place
+    next = steps && first < entries ? sel[first] : -1;
+    float w_next = w && steps && first < entries ? w[first] : 0.0f;
     for (int j = 0; j < steps; j++) {
-        const int i = first + j * 128 + lane * 4;
-        const int4 v = load(i);
-        const int a[4] = {v.x, v.y, v.z, v.w};
-        const uint32_t below = (1u << lane) - 1;
-        int at = base, mine = 0;
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-            const uint32_t m = __ballot_sync(0xffffffffu, a[c] == e);
-            at += __popc(m & below);
-            mine += __popc(m);
+        const int e = next;
+        const float we = w_next;
+        const int64_t i = first + j * 32;
+        if (j + 1 < steps) {
+            next = i + 32 < entries ? sel[i + 32] : -1;
+            if (w) w_next = i + 32 < entries ? w[i + 32] : 0.0f;
         }
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-            if (a[c] != e) continue;
-            slots[at] = i + c;
-            rows[at] = (i + c) / topk;
-            if (w_out) w_out[at] = w[i + c];
-            at++;
+        const bool own = (uint32_t)e < (uint32_t)E;
+        if (own) atomicOr(&mask[e], 1u << lane);
+        __syncwarp();
+        uint32_t same = 0;
+        if (own) {
+            same = mask[e];
+            const int at = place[e] + count[e] + __popc(same & below);
+            slots[at] = (int)i;
+            rows[at] = (int)i / topk;
+            if (w_out) w_out[at] = we;
         }
-        base += mine;
+        __syncwarp();
+        if (own && !(same & below)) {
+            count[e] += __popc(same);
+            mask[e] = 0;
+        }
+        __syncwarp();
     }
+    if (CLUSTER > 1) lists_cluster_sync();  // no block leaves while another may still read its totals
+}
+
+void lists_set_attributes() {
+    const int most = (2 * kListCounters + 2 * INZG_MAX_GROUPS) * (int)sizeof(int);
+    cudaFuncSetAttribute(expert_lists_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    cudaFuncSetAttribute(expert_lists_kernel<kListCluster>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
 }
 
 int launch_expert_lists(int n, int topk, int E, const int32_t *sel, const float *w, int32_t *off, int32_t *rows,
                         int32_t *slots, float *w_out, int32_t *err, cudaStream_t st) {
     const int entries = n * topk;
-    const int warps = std::max(1, std::min(kListWarps, (entries + 127) / 128));
-    if (reinterpret_cast<uintptr_t>(sel) & 15)
-        expert_lists_kernel<false><<<E, warps * 32, 0, st>>>(sel, w, entries, topk, E, off, rows, slots, w_out, err);
-    else
-        expert_lists_kernel<true><<<E, warps * 32, 0, st>>>(sel, w, entries, topk, E, off, rows, slots, w_out, err);
+    const int cluster = entries > 2048 ? kListCluster : 1;
+    const int warps = std::max(1, std::min({kListThreads / 32, kListCounters / E, (entries + cluster * 32 - 1) / (cluster * 32)}));
+    const size_t smem = sizeof(int) * (2 * (size_t)warps * E + 2 * (size_t)E);
+    if (cluster == 1) {
+        expert_lists_kernel<1><<<1, warps * 32, smem, st>>>(sel, w, entries, topk, E, off, rows, slots, w_out, err);
+        return 1;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(kListCluster);
+    cfg.blockDim = dim3(warps * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = kListCluster;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, expert_lists_kernel<kListCluster>, sel, w, entries, topk, E, off, rows, slots, w_out, err);
     return 1;
 }
 

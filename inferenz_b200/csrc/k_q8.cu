@@ -11,68 +11,79 @@
 
 namespace inzg {
 
-// One row per block; thread t holds chunks t, t + blockDim, ... (NCH of them, 8 columns each).
+// A block walks rows blockIdx.x, blockIdx.x + gridDim.x, ...; thread t holds chunks t, t + blockDim, ... of a row (NCH of them, 8
+// columns each). Up to 8192 columns it keeps their weights, and the next row's x and res are in flight while the current one is
+// reduced and written; wider rows (NCH = 4, up to 1024 threads of 64 registers) load both when they are due.
 template <class T, int NCH, bool VEC>
-__global__ void __launch_bounds__(1024) rmsnorm_q8_kernel(const inzg_rmsnorm_q8_args A) {
-    __shared__ float part[32];
-    const int64_t row = blockIdx.x;
-    const int cols = A.cols, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const T *x = static_cast<const T *>(A.x) + row * A.ldx;
-    const T *res = A.res ? static_cast<const T *>(A.res) + row * A.ldres : nullptr;
-    T *sum = A.sum ? static_cast<T *>(A.sum) + row * A.ldsum : nullptr;
-    float h[NCH][8];
-    float ss = 0.0f;
-#pragma unroll
-    for (int j = 0; j < NCH; j++) {
+__global__ void __launch_bounds__(NCH > 2 ? 1024 : 512) rmsnorm_q8_kernel(const inzg_rmsnorm_q8_args A) {
+    constexpr bool AHEAD = NCH <= 2;
+    __shared__ float part[2][32];
+    const int cols = A.cols, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    Chunk<T> x[AHEAD ? NCH : 1], r[AHEAD ? NCH : 1];
+    auto load_part = [&](int64_t row, int j, int to) {
         const int c = (threadIdx.x + j * blockDim.x) * 8, left = cols - c;
-        if (left > 0) load_chunk<T, VEC>(x + c, left, h[j]);
-        else
+        load_raw<T, VEC>(static_cast<const T *>(A.x) + row * A.ldx + c, left, x[to]);
+        if (A.res) load_raw<T, VEC>(static_cast<const T *>(A.res) + row * A.ldres + c, left, r[to]);
+    };
+    auto load_row = [&](int64_t row) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) h[j][i] = 0.0f;
-    }
-    if (res) {
+        for (int j = 0; j < NCH; j++) load_part(row, j, AHEAD ? j : 0);
+    };
+    if (AHEAD) load_row(blockIdx.x);
+    float w[AHEAD ? NCH : 1][8];
+    auto load_w = [&](int j, float(&o)[8]) {
+        const int c = (threadIdx.x + j * blockDim.x) * 8;
+        load_chunk<float, VEC>(A.w + c, cols - c, o);
+    };
+    if (AHEAD)
+#pragma unroll
+        for (int j = 0; j < NCH; j++) load_w(j, w[AHEAD ? j : 0]);
+    int flip = 0;
+    for (int64_t row = blockIdx.x; row < A.n; row += gridDim.x, flip ^= 1) {
+        float h[NCH][8], ss = 0.0f;
 #pragma unroll
         for (int j = 0; j < NCH; j++) {
-            const int c = (threadIdx.x + j * blockDim.x) * 8, left = cols - c;
-            if (left <= 0) continue;
-            float r[8];
-            load_chunk<T, VEC>(res + c, left, r);
+            const int jj = AHEAD ? j : 0;
+            if (!AHEAD) load_part(row, j, jj);
 #pragma unroll
-            for (int i = 0; i < 8; i++) h[j][i] += r[i];
+            for (int i = 0; i < 8; i++) {
+                h[j][i] = to_f32(x[jj].v[i]);
+                if (A.res) h[j][i] += to_f32(r[jj].v[i]);
+                ss = fmaf(h[j][i], h[j][i], ss);
+            }
         }
-    }
+        if (AHEAD && row + gridDim.x < A.n) load_row(row + gridDim.x);
+        if (A.sum)
 #pragma unroll
-    for (int j = 0; j < NCH; j++) {
-        const int c = (threadIdx.x + j * blockDim.x) * 8, left = cols - c;
-        if (sum && left > 0) store_chunk<T, VEC>(sum + c, left, h[j]);
+            for (int j = 0; j < NCH; j++) {
+                const int c = (threadIdx.x + j * blockDim.x) * 8, left = cols - c;
+                if (left > 0) store_chunk<T, VEC>(static_cast<T *>(A.sum) + row * A.ldsum + c, left, h[j]);
+            }
 #pragma unroll
-        for (int i = 0; i < 8; i++) ss = fmaf(h[j][i], h[j][i], ss);
-    }
+        for (int d = 16; d; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+        if (warps > 1) {
+            if (lane == 0) part[flip][warp] = ss;
+            __syncthreads();  // the other half of `part` is free: its readers have passed this barrier
+            ss = lane < warps ? part[flip][lane] : 0.0f;
 #pragma unroll
-    for (int d = 16; d; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-    if (lane == 0) part[warp] = ss;
-    __syncthreads();
-    ss = lane < (int)(blockDim.x >> 5) ? part[lane] : 0.0f;
+            for (int d = 16; d; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+        }
+        const float rs = __frcp_rn(__fsqrt_rn(__fdiv_rn(ss, (float)cols) + A.eps));
 #pragma unroll
-    for (int d = 16; d; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-    const float r = __frcp_rn(__fsqrt_rn(__fdiv_rn(ss, (float)cols) + A.eps));
+        for (int j = 0; j < NCH; j++) {
+            const int chunk = threadIdx.x + j * blockDim.x, c = chunk * 8, left = cols - c;
+            float v[8], (&wj)[8] = w[AHEAD ? j : 0];
+            if (!AHEAD) load_w(j, wj);
 #pragma unroll
-    for (int j = 0; j < NCH; j++) {
-        const int chunk = threadIdx.x + j * blockDim.x, c = chunk * 8, left = cols - c;
-        float v[8];
-        if (left > 0) load_chunk<float, VEC>(A.w + c, left, v);
-        else
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = left > i ? h[j][i] * r * v[i] : 0.0f;
-        if (A.y && left > 0) store_chunk<T, VEC>(static_cast<T *>(A.y) + row * A.ldy + c, left, v);
-        if (A.q) {
-            float s;
-            const uint2 q = quantize_chunk(v, s);
-            if (left > 0) {
-                store_q<VEC>(static_cast<uint8_t *>(A.q) + row * A.ldq + c, left, q);
-                if ((chunk & 15) == 0) A.s[row * A.lds + (chunk >> 4)] = s;
+            for (int i = 0; i < 8; i++) v[i] = left > i ? h[j][i] * rs * wj[i] : 0.0f;
+            if (A.y && left > 0) store_chunk<T, VEC>(static_cast<T *>(A.y) + row * A.ldy + c, left, v);
+            if (A.q) {
+                float s;
+                const uint2 q = quantize_chunk(v, s);
+                if (left > 0) {
+                    store_q<VEC>(static_cast<uint8_t *>(A.q) + row * A.ldq + c, left, q);
+                    if ((chunk & 15) == 0) A.s[row * A.lds + (chunk >> 4)] = s;
+                }
             }
         }
     }
@@ -88,32 +99,49 @@ __device__ __forceinline__ float exp_carried(float x) {
     return fabsf(t) < 160.0f ? fmaf(e, lo * 0.6931471805599453f, e) : e;  // past that e is 0, inf or NaN already
 }
 
-// A thread's slot: one chunk of one row; slots per row are rounded up to whole blocks of 128 columns.
+// A thread's slot: one chunk of one row; slots per row are rounded up to whole blocks of 128 columns. A thread goes on by
+// `step_rows` rows and `step_chunks` chunks, the grid's size in slots, and has the next slot's loads in flight.
 template <class T, bool VEC>
-__global__ void __launch_bounds__(256) silu_mul_q8_kernel(const inzg_silu_mul_q8_args A, uint32_t slots, uint32_t per_row) {
+__global__ void __launch_bounds__(256) silu_mul_q8_kernel(const inzg_silu_mul_q8_args A, uint32_t slots, uint32_t per_row,
+                                                          uint32_t step_rows, uint32_t step_chunks) {
     const int cols = A.cols;
-    // whole warps stay in the loop: the quantizer shuffles
-    for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i - threadIdx.x % 32 < slots; i += gridDim.x * blockDim.x) {
-        const uint32_t row = i / per_row, chunk = i % per_row;
+    uint32_t i = blockIdx.x * blockDim.x + threadIdx.x, row = i / per_row, chunk = i % per_row;
+    Chunk<T> g, u;
+    auto load = [&] {
         const int c = (int)chunk * 8, left = i < slots ? cols - c : 0;
-        float g[8], u[8];
-        if (left > 0) {
-            const T *x = static_cast<const T *>(A.x) + (int64_t)row * A.ldx;
-            load_chunk<T, VEC>(x + c, left, g);
-            load_chunk<T, VEC>(x + cols + c, left, u);
-        } else {
+        const T *x = static_cast<const T *>(A.x) + (int64_t)row * A.ldx + c;
+        load_raw<T, VEC>(x, left, g);
+        load_raw<T, VEC>(x + cols, left, u);
+    };
+    load();
+    // whole warps stay in the loop: the quantizer shuffles
+    while (i - threadIdx.x % 32 < slots) {
+        const int c = (int)chunk * 8, left = i < slots ? cols - c : 0;
+        const bool first = (chunk & 15) == 0;
+        const int64_t r = row, block = chunk >> 4;
+        float v[8], gate[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) g[j] = u[j] = 0.0f;
+        for (int j = 0; j < 8; j++) {
+            gate[j] = to_f32(g.v[j]);
+            v[j] = to_f32(u.v[j]);
         }
+        i += gridDim.x * blockDim.x;
+        row += step_rows;
+        chunk += step_chunks;
+        if (chunk >= per_row) {
+            chunk -= per_row;
+            row++;
+        }
+        load();
 #pragma unroll
-        for (int j = 0; j < 8; j++) u[j] *= __fdividef(g[j], 1.0f + exp_carried(-g[j]));
-        if (A.y && left > 0) store_chunk<T, VEC>(static_cast<T *>(A.y) + (int64_t)row * A.ldy + c, left, u);
+        for (int j = 0; j < 8; j++) v[j] *= __fdividef(gate[j], 1.0f + exp_carried(-gate[j]));
+        if (A.y && left > 0) store_chunk<T, VEC>(static_cast<T *>(A.y) + r * A.ldy + c, left, v);
         if (A.q) {
             float s;
-            const uint2 q = quantize_chunk(u, s);
+            const uint2 q = quantize_chunk(v, s);
             if (left > 0) {
-                store_q<VEC>(static_cast<uint8_t *>(A.q) + (int64_t)row * A.ldq + c, left, q);
-                if ((chunk & 15) == 0) A.s[(int64_t)row * A.lds + (chunk >> 4)] = s;
+                store_q<VEC>(static_cast<uint8_t *>(A.q) + r * A.ldq + c, left, q);
+                if (first) A.s[r * A.lds + block] = s;
             }
         }
     }
@@ -131,15 +159,16 @@ static int norm_typed(const inzg_rmsnorm_q8_args &A, int num_sms, cudaStream_t s
     const bool vec = aligned(A.x, A.ldx * b, 16) && aligned(A.res, A.ldres * b, 16) && aligned(A.sum, A.ldsum * b, 16) &&
                      aligned(A.y, A.ldy * b, 16) && aligned(A.q, A.ldq, 8) && aligned(A.w, 0, 16);
     const int chunks = (A.cols + 7) / 8;
-    // few rows: one chunk per thread, the shortest chain; many: two, so that a block holds fewer warps and more rows are
-    // in flight; wide rows as many as 1024 threads need
-    int nch = A.n <= num_sms ? 1 : 2;
-    while (nch < 4 && chunks > nch * 1024) nch *= 2;
+    // few rows: one chunk per thread, the shortest chain; many: two, so that a block's warps have more of a row each; wide rows as
+    // many as 1024 threads need
+    int nch = A.n <= num_sms && chunks <= 512 ? 1 : chunks <= 1024 ? 2 : 4;
     const int threads = ((chunks + nch - 1) / nch + 31) / 32 * 32;
+    const int per_sm = threads > 512 ? 1 : 1024 / threads;  // blocks that an SM holds with their next rows in registers
+    const int grid = (int)(A.n < (int64_t)num_sms * per_sm ? A.n : num_sms * per_sm);
 #define INZG_NORM(NCH)                                                                                        \
     do {                                                                                                      \
-        if (vec) rmsnorm_q8_kernel<T, NCH, true><<<A.n, threads, 0, st>>>(A);                                 \
-        else rmsnorm_q8_kernel<T, NCH, false><<<A.n, threads, 0, st>>>(A);                                    \
+        if (vec) rmsnorm_q8_kernel<T, NCH, true><<<grid, threads, 0, st>>>(A);                                \
+        else rmsnorm_q8_kernel<T, NCH, false><<<grid, threads, 0, st>>>(A);                                   \
     } while (0)
     if (nch == 1) INZG_NORM(1);
     else if (nch == 2) INZG_NORM(2);
@@ -177,10 +206,10 @@ static int silu_typed(inzg_silu_mul_q8_args A, int num_sms, cudaStream_t st) {
         if (A.q) P.q = static_cast<uint8_t *>(A.q) + done * A.ldq;
         if (A.s) P.s = A.s + done * A.lds;
         const uint32_t slots = (uint32_t)P.n * per_row;
-        const uint32_t want = (slots + 255) / 256, most = (uint32_t)num_sms * 8;
-        const uint32_t grid = want < most ? want : most;
-        if (vec) silu_mul_q8_kernel<T, true><<<grid, 256, 0, st>>>(P, slots, per_row);
-        else silu_mul_q8_kernel<T, false><<<grid, 256, 0, st>>>(P, slots, per_row);
+        const uint32_t want = (slots + 255) / 256, most = (uint32_t)num_sms * 6;
+        const uint32_t grid = want < most ? want : most, step = grid * 256;
+        if (vec) silu_mul_q8_kernel<T, true><<<grid, 256, 0, st>>>(P, slots, per_row, step / per_row, step % per_row);
+        else silu_mul_q8_kernel<T, false><<<grid, 256, 0, st>>>(P, slots, per_row, step / per_row, step % per_row);
         launches++;
     }
     return launches;

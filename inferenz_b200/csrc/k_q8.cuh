@@ -55,6 +55,21 @@ __device__ __forceinline__ void load_chunk(const T *p, int left, float (&o)[8]) 
     }
 }
 
+// the same as it lies in memory (behind the row: zeros)
+template <class T, bool VEC>
+__device__ __forceinline__ void load_raw(const T *p, int left, Chunk<T> &o) {
+    if (VEC && left >= 8) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(o) / 16; i++) reinterpret_cast<uint4 *>(&o)[i] = reinterpret_cast<const uint4 *>(p)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (i < left) o.v[i] = p[i];
+            else from_f32(0.0f, o.v[i]);
+        }
+    }
+}
+
 template <class T, bool VEC>
 __device__ __forceinline__ void store_chunk(T *p, int left, const float (&v)[8]) {
     Chunk<T> c;
@@ -88,7 +103,10 @@ __device__ __forceinline__ uint2 quantize_chunk(const float (&v)[8], float &s) {
     for (int i = 0; i < 8; i++) a = fmaxf(a, fabsf(v[i]));
 #pragma unroll
     for (int d = 8; d; d >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, d));
-    s = __fdiv_rn(a, kE4m3Max);
+    // a / 448, rounded to nearest: the product with 1 / 448 and one correction by its remainder
+    const float t = a * (1.0f / kE4m3Max);
+    s = fmaf(fmaf(-kE4m3Max, t, a), 1.0f / kE4m3Max, t);
+    if (!(s < __int_as_float(0x7F800000))) s = a;  // an infinity has no remainder
     const float inv = __frcp_rn(s);
     uint2 q;
     q.x = cvt_e4m3x2(v[0] * inv, v[1] * inv) | cvt_e4m3x2(v[2] * inv, v[3] * inv) << 16;
