@@ -89,15 +89,20 @@ __global__ void __launch_bounds__(NCH > 2 ? 1024 : 512) rmsnorm_q8_kernel(const 
     }
 }
 
-// exp(x) for x in fp32: 2^(x log2 e) with the product's rounding error carried to first order, so that the relative error
-// stays at a few 2^-24 for large |x| too, where the hardware's 2^t on the rounded product alone loses |x| * 2^-24.
+// exp(x) for |x| <= 88, x clamped to that: 2^(x log2 e) with the product's rounding error carried to first order, so that the
+// relative error stays at a few 2^-24 for large |x| too, where the hardware's 2^t on the rounded product alone loses |x| * 2^-24.
 __device__ __forceinline__ float exp_carried(float x) {
+    x = fminf(fmaxf(x, -88.0f), 88.0f);
     const float t = x * 1.4426950408889634f;
-    const float lo = fmaf(x, 1.4426950408889634f, -t) + x * 1.925963033500938e-8f;  // log2 e = hi + 1.926e-8
+    const float lo = fmaf(x, 1.925963033500938e-8f, fmaf(x, 1.4426950408889634f, -t));  // log2 e = hi + 1.926e-8
     float e;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-    return fabsf(t) < 160.0f ? fmaf(e, lo * 0.6931471805599453f, e) : e;  // past that e is 0, inf or NaN already
+    return fmaf(e, lo * 0.6931471805599453f, e);
 }
+
+// g / (1 + exp(-g)). Below -87.3 the divisor passes 2^126 and the fast division gives 0 (or NaN for -infinity); the true value is
+// less than 2^-119 there. A NaN passes through the product.
+__device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.0f + exp_carried(-g)); }
 
 // A thread's slot: one chunk of one row; slots per row are rounded up to whole blocks of 128 columns. A thread goes on by
 // `step_rows` rows and `step_chunks` chunks, the grid's size in slots, and has the next slot's loads in flight.
@@ -134,7 +139,7 @@ __global__ void __launch_bounds__(256) silu_mul_q8_kernel(const inzg_silu_mul_q8
         }
         load();
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] *= __fdividef(gate[j], 1.0f + exp_carried(-gate[j]));
+        for (int j = 0; j < 8; j++) v[j] *= silu(gate[j]);
         if (A.y && left > 0) store_chunk<T, VEC>(static_cast<T *>(A.y) + r * A.ldy + c, left, v);
         if (A.q) {
             float s;
@@ -156,12 +161,10 @@ static bool aligned(const void *p, int64_t ld_bytes, int to) {
 template <class T>
 static int norm_typed(const inzg_rmsnorm_q8_args &A, int num_sms, cudaStream_t st) {
     const int64_t b = sizeof(T);
-    const bool vec = aligned(A.x, A.ldx * b, 16) && aligned(A.res, A.ldres * b, 16) && aligned(A.sum, A.ldsum * b, 16) &&
+    const bool vec = A.cols % 8 == 0 && aligned(A.x, A.ldx * b, 16) && aligned(A.res, A.ldres * b, 16) && aligned(A.sum, A.ldsum * b, 16) &&
                      aligned(A.y, A.ldy * b, 16) && aligned(A.q, A.ldq, 8) && aligned(A.w, 0, 16);
     const int chunks = (A.cols + 7) / 8;
-    // few rows: one chunk per thread, the shortest chain; many: two, so that a block's warps have more of a row each; wide rows as
-    // many as 1024 threads need
-    int nch = A.n <= num_sms && chunks <= 512 ? 1 : chunks <= 1024 ? 2 : 4;
+    const int nch = chunks <= 512 ? 1 : chunks <= 1024 ? 2 : 4;  // chunks per thread
     const int threads = ((chunks + nch - 1) / nch + 31) / 32 * 32;
     const int per_sm = threads > 512 ? 1 : 1024 / threads;  // blocks that an SM holds with their next rows in registers
     const int grid = (int)(A.n < (int64_t)num_sms * per_sm ? A.n : num_sms * per_sm);
@@ -193,7 +196,7 @@ int launch_rmsnorm_q8(const inzg_rmsnorm_q8_args &args, int num_sms, cudaStream_
 template <class T>
 static int silu_typed(inzg_silu_mul_q8_args A, int num_sms, cudaStream_t st) {
     const int64_t b = sizeof(T);
-    const bool vec = aligned(A.x, A.ldx * b, 16) && aligned(A.x, A.cols * b, 16) && aligned(A.y, A.ldy * b, 16) &&
+    const bool vec = A.cols % 8 == 0 && aligned(A.x, A.ldx * b, 16) && aligned(A.y, A.ldy * b, 16) &&
                      aligned(A.q, A.ldq, 8);
     const uint32_t per_row = (uint32_t)(A.cols + kQB - 1) / kQB * 16;
     const int rows_max = (int)(0x40000000u / per_row);  // slots are counted in 32 bits: more rows take more launches

@@ -39,7 +39,8 @@ struct alignas(16) Chunk {
     T v[8];
 };
 
-// the chunk at p as fp32; VEC: p is 16-byte aligned. `left`: elements of the row from p on (what lies behind reads 0)
+// the chunk at p as fp32. `left`: elements of the row from p on (what lies behind reads 0). VEC: p is 16-byte aligned and a row a
+// multiple of 8 elements, so a chunk lies inside or behind it
 template <class T, bool VEC>
 __device__ __forceinline__ void load_chunk(const T *p, int left, float (&o)[8]) {
     if (VEC && left >= 8) {
@@ -51,7 +52,7 @@ __device__ __forceinline__ void load_chunk(const T *p, int left, float (&o)[8]) 
         for (int i = 0; i < 8; i++) o[i] = to_f32(c.v[i]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) o[i] = i < left ? to_f32(p[i]) : 0.0f;
+        for (int i = 0; i < 8; i++) o[i] = !VEC && i < left ? to_f32(p[i]) : 0.0f;
     }
 }
 
@@ -64,7 +65,7 @@ __device__ __forceinline__ void load_raw(const T *p, int left, Chunk<T> &o) {
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            if (i < left) o.v[i] = p[i];
+            if (!VEC && i < left) o.v[i] = p[i];
             else from_f32(0.0f, o.v[i]);
         }
     }
@@ -79,7 +80,7 @@ __device__ __forceinline__ void store_chunk(T *p, int left, const float (&v)[8])
 #pragma unroll
         for (int i = 0; i < (int)sizeof(c) / 16; i++)
             reinterpret_cast<uint4 *>(p)[i] = reinterpret_cast<const uint4 *>(&c)[i];
-    } else {
+    } else if (!VEC) {
 #pragma unroll
         for (int i = 0; i < 8; i++)
             if (i < left) p[i] = c.v[i];
@@ -94,9 +95,9 @@ __device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
 }
 
 // s = max(max |v|, 2^-100) / 448 over the 16 lanes of a block (every lane of the warp calls it), q = e4m3(v / s) of this
-// lane's 8. v / s is taken as v * (1 / s), both correctly rounded: within 2^-23 of the quotient, so a value whose quotient
-// lies that near a border of two e4m3 values may fall to the other side. fmaxf drops NaN, so the others keep a scale;
-// an infinity makes s infinite and 1 / s zero: its own place becomes NaN and the block reads as NaN.
+// lane's 8. v / s is taken as v * (1 / s): within 2^-23 of the quotient, so a value whose quotient lies that near a border of two
+// e4m3 values may fall to the other side. fmaxf drops NaN, so the others keep a scale; an infinity makes s infinite and every
+// value of the block NaN.
 __device__ __forceinline__ uint2 quantize_chunk(const float (&v)[8], float &s) {
     float a = kAmaxFloor;
 #pragma unroll
@@ -107,7 +108,10 @@ __device__ __forceinline__ uint2 quantize_chunk(const float (&v)[8], float &s) {
     const float t = a * (1.0f / kE4m3Max);
     s = fmaf(fmaf(-kE4m3Max, t, a), 1.0f / kE4m3Max, t);
     if (!(s < __int_as_float(0x7F800000))) s = a;  // an infinity has no remainder
-    const float inv = __frcp_rn(s);
+    // 1 / s: the hardware's estimate and one Newton step (s is a normal number with a normal reciprocal, or infinite)
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    inv = fmaf(fmaf(-s, inv, 1.0f), inv, inv);
     uint2 q;
     q.x = cvt_e4m3x2(v[0] * inv, v[1] * inv) | cvt_e4m3x2(v[2] * inv, v[3] * inv) << 16;
     q.y = cvt_e4m3x2(v[4] * inv, v[5] * inv) | cvt_e4m3x2(v[6] * inv, v[7] * inv) << 16;
@@ -118,7 +122,7 @@ template <bool VEC>
 __device__ __forceinline__ void store_q(uint8_t *p, int left, uint2 q) {
     if (VEC && left >= 8) {
         *reinterpret_cast<uint2 *>(p) = q;
-    } else {
+    } else if (!VEC) {
 #pragma unroll
         for (int i = 0; i < 8; i++)
             if (i < left) p[i] = (uint8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
