@@ -305,13 +305,18 @@ template <int TN>
 constexpr size_t gmm_smem() {
     return (size_t)GmmCfg<TN>::kStages * GmmCfg<TN>::kStage + sizeof(GmmShared<TN>) + 1024;
 }
-static_assert(gmm_smem<32>() <= 227 * 1024 && gmm_smem<128>() <= 227 * 1024, "shared memory of one CTA");
+// more than half of an SM's shared memory, so that a CTA is alone on its SM with all of TMEM
+static_assert(gmm_smem<32>() <= 227 * 1024 && gmm_smem<32>() > 116 * 1024, "one CTA per SM");
+static_assert(gmm_smem<128>() <= 227 * 1024 && gmm_smem<128>() > 116 * 1024, "one CTA per SM");
+static bool g_wide_ok = false, g_large_ok = false;  // the kernels with a register split may be launched
 
 void gmm_set_attributes() {
     cudaFuncSetAttribute(gmm_kernel<true, 32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)gmm_smem<32>());
     cudaFuncSetAttribute(gmm_kernel<false, 32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)gmm_smem<32>());
-    cudaFuncSetAttribute(gmm_kernel<false, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)gmm_smem<128>());
-    gmm_large_set_attributes();
+    g_wide_ok = cudaFuncSetAttribute(gmm_kernel<false, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)gmm_smem<128>()) ==
+                    cudaSuccess &&
+                gmm_split_holds(gmm_kernel<false, 128>);
+    g_large_ok = gmm_large_set_attributes();
 }
 
 template <bool F8, int TN>
@@ -361,11 +366,12 @@ int launch_grouped_matmul(const inzg_grouped_matmul_args &G, int num_sms, int32_
     //   e4m3, 8 groups:     64 a group: 32-entry tiles 15, 128 x 256 tiles 20; 128 a group: 21, 20
     // The last case has fewer large tiles than half the SMs, and small ones fill the GPU better.
     if (G.type != INZG_T_E4M3) {
-        if (G.entries <= 24 * (int64_t)G.groups) return gmm_launch<false, 32>(G, A, num_sms, st);
+        if (G.entries <= 24 * (int64_t)G.groups || !g_wide_ok) return gmm_launch<false, 32>(G, A, num_sms, st);
         return gmm_launch<false, 128>(G, A, num_sms, st);
     }
     const int64_t large_items = std::min<int64_t>(G.entries, G.entries / 128 + G.groups) * ((G.n + 255) / 256);
-    if (G.entries <= (large_items <= num_sms / 2 ? 96 : 48) * (int64_t)G.groups) return gmm_launch<true, 32>(G, A, num_sms, st);
+    if (G.entries <= (large_items <= num_sms / 2 ? 96 : 48) * (int64_t)G.groups || !g_large_ok)
+        return gmm_launch<true, 32>(G, A, num_sms, st);
     return gmm_large_launch(G, A, num_sms, st);
 }
 

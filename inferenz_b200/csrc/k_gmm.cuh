@@ -406,8 +406,17 @@ __device__ __forceinline__ bool gmm_stage_walk(GmmStaged<TILE, TEAMS, PLANES, KC
 // outside reads as zeros. False when the driver refuses it.
 bool gmm_map(CUtensorMap *m, const void *base, int elem, int64_t rows, int64_t k, int64_t ld, int box_rows);
 
-// The two kernels' launchers (k_gmm.cu, k_gmm_large.cu): A holds everything but nrb and the tile-dependent bits
-void gmm_large_set_attributes();
+// Kernels that hand registers from some warps to others (setmaxnreg) need the 128 per thread at launch that their split adds up
+// to, or the receiving warps wait for ever: whether `kernel` was built with them.
+template <class F>
+inline bool gmm_split_holds(F kernel) {
+    cudaFuncAttributes at{};
+    return cudaFuncGetAttributes(&at, kernel) == cudaSuccess && at.numRegs == 128;
+}
+
+// The kernel for many entries (k_gmm_large.cu): A holds everything but nrb and the tile-dependent bits. The attributes' call returns
+// false when the kernel may not be launched.
+bool gmm_large_set_attributes();
 int gmm_large_launch(const inzg_grouped_matmul_args &G, GmmArgs A, int num_sms, cudaStream_t st);
 
 }  // namespace inzg

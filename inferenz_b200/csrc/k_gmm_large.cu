@@ -267,10 +267,12 @@ gmm_large_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 // ---------------------------------------------------------------------------------------------------------------------
 
 constexpr size_t kLargeSmem = (size_t)LSTAGES * kLargeStage + sizeof(LargeShared) + 1024;
-static_assert(kLargeSmem <= 227 * 1024, "shared memory of one CTA");
+// more than half of an SM's shared memory, so that a CTA is alone on its SM with all of TMEM
+static_assert(kLargeSmem <= 227 * 1024 && kLargeSmem > 116 * 1024, "one CTA per SM");
 
-void gmm_large_set_attributes() {
-    cudaFuncSetAttribute(gmm_large_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kLargeSmem);
+bool gmm_large_set_attributes() {
+    return cudaFuncSetAttribute(gmm_large_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kLargeSmem) == cudaSuccess &&
+           gmm_split_holds(gmm_large_kernel);
 }
 
 int gmm_large_launch(const inzg_grouped_matmul_args &G, GmmArgs A, int num_sms, cudaStream_t st) {

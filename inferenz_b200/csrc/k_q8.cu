@@ -76,10 +76,13 @@ __global__ void __launch_bounds__(NCH > 2 ? 1024 : 512) rmsnorm_q8_kernel(const 
             if (!AHEAD) load_w(j, wj);
 #pragma unroll
             for (int i = 0; i < 8; i++) v[i] = left > i ? h[j][i] * rs * wj[i] : 0.0f;
+            float z[8];  // v without the row's factor
+#pragma unroll
+            for (int i = 0; i < 8; i++) z[i] = left > i ? h[j][i] * wj[i] : 0.0f;
             if (A.y && left > 0) store_chunk<T, VEC>(static_cast<T *>(A.y) + row * A.ldy + c, left, v);
             if (A.q) {
                 float s;
-                const uint2 q = quantize_chunk(v, s);
+                const uint2 q = quantize_scaled(z, v, rs, s);
                 if (left > 0) {
                     store_q<VEC>(static_cast<uint8_t *>(A.q) + row * A.ldq + c, left, q);
                     if ((chunk & 15) == 0) A.s[row * A.lds + (chunk >> 4)] = s;

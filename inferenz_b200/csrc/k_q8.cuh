@@ -94,27 +94,61 @@ __device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
     return r;
 }
 
+// max of `least` and |v| over the 16 lanes of a block (every lane of the warp calls it; NaN is dropped)
+__device__ __forceinline__ float block_amax(const float (&v)[8], float least) {
+    float a = least;
+#pragma unroll
+    for (int i = 0; i < 8; i++) a = fmaxf(a, fabsf(v[i]));
+#pragma unroll
+    for (int d = 8; d; d >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, d));
+    return a;
+}
+
+// a / 448, rounded to nearest: the product with 1 / 448 and one correction by its remainder (an infinity has none)
+__device__ __forceinline__ float scale_of(float a) {
+    const float t = a * (1.0f / kE4m3Max);
+    const float s = fmaf(fmaf(-kE4m3Max, t, a), 1.0f / kE4m3Max, t);
+    return s < __int_as_float(0x7F800000) ? s : a;
+}
+
+__device__ __forceinline__ float rcp_approx(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// 8 products as e4m3
+__device__ __forceinline__ uint2 e4m3_times(const float (&v)[8], float f) {
+    uint2 q;
+    q.x = cvt_e4m3x2(v[0] * f, v[1] * f) | cvt_e4m3x2(v[2] * f, v[3] * f) << 16;
+    q.y = cvt_e4m3x2(v[4] * f, v[5] * f) | cvt_e4m3x2(v[6] * f, v[7] * f) << 16;
+    return q;
+}
+
 // s = max(max |v|, 2^-100) / 448 over the 16 lanes of a block (every lane of the warp calls it), q = e4m3(v / s) of this
 // lane's 8. v / s is taken as v * (1 / s): within 2^-23 of the quotient, so a value whose quotient lies that near a border of two
 // e4m3 values may fall to the other side. fmaxf drops NaN, so the others keep a scale; an infinity makes s infinite and every
 // value of the block NaN.
 __device__ __forceinline__ uint2 quantize_chunk(const float (&v)[8], float &s) {
-    float a = kAmaxFloor;
-#pragma unroll
-    for (int i = 0; i < 8; i++) a = fmaxf(a, fabsf(v[i]));
-#pragma unroll
-    for (int d = 8; d; d >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, d));
-    // a / 448, rounded to nearest: the product with 1 / 448 and one correction by its remainder
-    const float t = a * (1.0f / kE4m3Max);
-    s = fmaf(fmaf(-kE4m3Max, t, a), 1.0f / kE4m3Max, t);
-    if (!(s < __int_as_float(0x7F800000))) s = a;  // an infinity has no remainder
+    s = scale_of(block_amax(v, kAmaxFloor));
     // 1 / s: the hardware's estimate and one Newton step (s is a normal number with a normal reciprocal, or infinite)
-    float inv;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    float inv = rcp_approx(s);
     inv = fmaf(fmaf(-s, inv, 1.0f), inv, inv);
-    uint2 q;
-    q.x = cvt_e4m3x2(v[0] * inv, v[1] * inv) | cvt_e4m3x2(v[2] * inv, v[3] * inv) << 16;
-    q.y = cvt_e4m3x2(v[4] * inv, v[5] * inv) | cvt_e4m3x2(v[6] * inv, v[7] * inv) << 16;
+    return e4m3_times(v, inv);
+}
+
+// The same for v = z * r with one r > 0 for the row, without r's error in the quotients: v / s = z * (448 / max |z|), the
+// factor rounded once. Where that leaves the normal range (and for blocks at the floor) v itself is quantized.
+__device__ __forceinline__ uint2 quantize_scaled(const float (&z)[8], const float (&v)[8], float r, float &s) {
+    const float a = block_amax(z, 0.0f);
+    const bool plain = a > 8.077935669463161e-28f && a < 8.507059173023462e37f && a * r > kAmaxFloor;  // 2^-90, 2^126
+    uint2 q = make_uint2(0, 0);
+    if (!__all_sync(0xffffffffu, plain)) q = quantize_chunk(v, s);
+    if (plain) {
+        s = scale_of(a * r);
+        const float t = rcp_approx(a), f = kE4m3Max * t;
+        q = e4m3_times(z, fmaf(fmaf(-f, a, kE4m3Max), t, f));
+    }
     return q;
 }
 

@@ -440,6 +440,39 @@ def test_grouped_real(pool, t, E, entries, n, k, out):
     assert bool(((o.double() - want).abs() <= bound)[wrote].all())
 
 
+@pytest.mark.parametrize("t,entries,n,k", [(T_E4M3, 2048 * 52, 9600, 16), (T_E4M3, 2048, 12_000, 16), (T_F16, 2048, 12_000, 8)])
+def test_grouped_many_items(pool, t, entries, n, k):
+    """more items per SM than the list that each CTA keeps of them (2048 groups x n / 256 or n / 128 row blocks over 148 SMs)"""
+    E, g = 2048, _gen(3)
+    off = torch.arange(E + 1, device="cuda", dtype=torch.int64) * entries // E
+    a, w = _ints(entries, k, 16, DT[t], g), _ints(E * n, k, 16, DT[t], g)
+    f8 = t == T_E4M3
+    sa, sw = (_pow2((entries, 1), g), _pow2((E, (n + 127) // 128, 1), g)) if f8 else (None, None)
+    o = torch.full((entries, n), CANARY, device="cuda", dtype=torch.bfloat16)
+    p = lambda x: x.data_ptr() if x is not None else None  # noqa: E731
+    off32 = off.to(torch.int32)
+    pool.grouped_matmul_device(t, E, n, k, entries, entries, p(a), p(w), p(off32), p(o), T_BF16, lda=16, ldw=16, a_scale_ptr=p(sa),
+                               w_scale_ptr=p(sw), stream=_st())
+    pool.device_status(_st())
+    cols = torch.randint(0, n, (40,), generator=g, device="cuda")
+    group = torch.searchsorted(off[1:], torch.arange(entries, device="cuda"), right=True)
+    for c in torch.cat([cols, torch.tensor([0, n - 1], device="cuda")]).tolist():
+        want = (a.float() * w.view(torch.uint8).view(E, n, -1)[:, c].contiguous().view(w.dtype).float()[group]).sum(1) if f8 else \
+            (a.float() * w.unflatten(0, (E, n))[:, c].float()[group]).sum(1)
+        if f8:
+            want = want * sa[:, 0] * sw[group, c // 128, 0]
+        assert torch.equal(o[:, c], want.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("t,m,k", [(T_E4M3, 5, 20_011), (T_E4M3, 300, 20_011), (T_BF16, 5, 10_003), (T_BF16, 300, 10_003)])
+def test_grouped_long_rows(pool, t, m, k):
+    """157 blocks of k: the rings and the staged scales go round many times"""
+    c = _grouped_case(t, 2, m, 200, k, True, True, m)
+    o, _ = _run_grouped(pool, t, c, 2, m, 200, k, T_F32)
+    want, _, wrote = _grouped_want(c, 2, m, 200)
+    assert float(want.abs().max()) < 2.0 ** 20 and torch.equal(o.double()[wrote], want[wrote])
+
+
 @pytest.mark.parametrize("t", [T_E4M3, T_BF16])
 def test_grouped_lists_inside_the_entries(pool, t):
     """offsets that begin after 0 and end before `entries`: what they leave out stays as it was"""
