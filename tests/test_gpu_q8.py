@@ -185,6 +185,18 @@ def test_silu_mul(pool, t, n, cols, pad, offset):
         _behind_is_untouched(buf, view)
 
 
+def test_silu_more_rows_than_one_launch_counts(pool):
+    """narrow rows: 2^26 and a few, counted in two launches"""
+    n = (1 << 26) + 5
+    x = torch.randn(n, 2, generator=_gen(8), device="cuda", dtype=torch.bfloat16)
+    y = torch.full((n, 1), CANARY, device="cuda", dtype=torch.bfloat16)
+    pool.silu_mul_q8_device(n, 1, T_BF16, x.data_ptr(), y_ptr=y.data_ptr(), stream=_st())
+    for at in (slice(0, 1000), slice(n // 2, n // 2 + 1000), slice(n - 1000, n)):
+        g, u = x[at, 0].double(), x[at, 1].double()
+        v = g * torch.sigmoid(g) * u
+        assert bool(((y[at, 0].double() - v).abs() <= (half_step(y.dtype) + 12 * U) * v.abs() * 1.01 + 1e-38).all())
+
+
 def test_silu_extremes(pool):
     """gates far out on both sides, infinities and NaN"""
     inf, nan = float("inf"), float("nan")
@@ -251,6 +263,23 @@ def test_expert_lists_of_one_expert_and_no_tokens(pool):
     off.fill_(9)
     pool.expert_lists_device(0, 3, 8, None, off.data_ptr(), None, None, stream=_st())
     assert off.tolist() == [0] * 9
+
+
+@pytest.mark.parametrize("n,K,E,kind", [(20_000, 10, 512, "random"), (3001, 3, 512, "one"), (2049, 1, 7, "two"), (700, 3, 9, "none"),
+                                        (4096, 8, 2048, "runs")])
+def test_expert_lists_long_and_skewed(pool, n, K, E, kind):
+    """past one block's entries: many of them, all of one expert, of two in turn, none on this rank, long runs"""
+    i = torch.arange(n * K, device="cuda")
+    sel = {"random": torch.randint(0, E, (n * K,), generator=_gen(4), device="cuda"), "one": torch.full_like(i, E - 1),
+           "two": (i % 2) * (E - 1), "none": torch.full_like(i, -1), "runs": i * E // (n * K)}[kind].to(torch.int32).view(n, K)
+    w = torch.rand(n, K, generator=_gen(5), device="cuda")
+    off, rows, slots, wo = _lists(pool, sel, E, w)
+    want_off, order = _lists_want(sel, E)
+    m = len(order)
+    assert np.array_equal(off.cpu().numpy(), want_off) and np.array_equal(slots.cpu().numpy()[:m], order)
+    assert np.array_equal(rows.cpu().numpy()[:m], order // K) and torch.equal(wo[:m], w.reshape(-1)[slots[:m].long()])
+    assert bool((slots[m:] == -7).all())
+    pool.device_status(_st())
 
 
 def test_expert_lists_report_a_bad_expert_once(pool):
@@ -568,6 +597,93 @@ def test_streams_and_graph(pool):
     torch.cuda.synchronize()
     check()
     pool.device_status(_st())
+
+
+@pytest.mark.parametrize("t", [T_E4M3, T_BF16])
+@pytest.mark.parametrize("entries", [7, 600])
+def test_grouped_with_no_listed_entries(pool, t, entries):
+    c = _grouped_case(t, 9, entries, 140, 256, True, True, 2)
+    c["off"].fill_(3)
+    o, _ = _run_grouped(pool, t, c, 9, entries, 140, 256, T_F32)
+    pool.device_status(_st())
+    assert bool((o == CANARY).all())
+
+
+def test_grouped_scale_pitch_and_repeated_rows(pool):
+    """scales with a pitch of their own; every entry of one group reads the same row of a"""
+    for entries in (20, 400):
+        E, n, k, g = 2, 200, 600, _gen(entries)
+        c = _grouped_case(T_E4M3, E, entries, n, k, True, False, 31)
+        c["in"].fill_(c["a"].shape[0] - 1)
+        wide = torch.full((c["a"].shape[0], 9), float("nan"), device="cuda")
+        wide[:, :5] = c["as"]
+        o = torch.empty(entries, n, device="cuda")
+        p = lambda x: x.data_ptr()  # noqa: E731
+        pool.grouped_matmul_device(T_E4M3, E, n, k, c["a"].shape[0], entries, p(c["a"]), p(c["w"]), p(c["off"]), p(o), T_F32,
+                                   lda=c["a"].stride(0), ldw=c["w"].stride(0), a_scale_ptr=p(wide), lda_scale=9,
+                                   w_scale_ptr=p(c["ws"]), in_rows_ptr=p(c["in"]), stream=_st())
+        want, _, wrote = _grouped_want(c, E, entries, n)
+        assert bool(wrote.all()) and torch.equal(o.double(), want)
+
+
+def test_every_operator_captured_and_replayed(pool):
+    """norm -> lists -> gate|up -> SiLU * up -> down in one graph; the replay on new contents of the same buffers gives what calls on
+    them give"""
+    n, H, FF, E, K, g = 300, 512, 256, 16, 4, _gen(12)
+    dt = torch.bfloat16
+    p = lambda x: x.data_ptr()  # noqa: E731
+    f8 = lambda r, k: (torch.randn(r, k, generator=g, device="cuda") * 120).clamp(-448, 448).to(F8)  # noqa: E731
+    x, res, w = torch.empty(n, H, dtype=dt, device="cuda"), torch.empty(n, H, dtype=dt, device="cuda"), torch.ones(H, device="cuda")
+    wg, wd = f8(E * 2 * FF, H), f8(E * H, FF)
+    sg, sd = torch.rand(E, 4, 4, generator=g, device="cuda") / 3000, torch.rand(E, 4, 2, generator=g, device="cuda") / 3000
+    sel, rw = torch.empty(n, K, dtype=torch.int32, device="cuda"), torch.rand(n, K, generator=g, device="cuda")
+    total, q, s = torch.empty_like(x), torch.empty(n, H, dtype=F8, device="cuda"), torch.empty(n, 4, device="cuda")
+    off, rows, slots = (torch.empty(m, dtype=torch.int32, device="cuda") for m in (E + 1, n * K, n * K))
+    lw, gu = torch.empty(n * K, device="cuda"), torch.empty(n * K, 2 * FF, dtype=dt, device="cuda")
+    hq, hs, out = torch.empty(n * K, FF, dtype=F8, device="cuda"), torch.empty(n * K, 2, device="cuda"), torch.empty(n * K, H, device="cuda")
+
+    def layer(st):
+        pool.rmsnorm_q8_device(n, H, T_BF16, p(x), p(w), 1e-6, res_ptr=p(res), sum_ptr=p(total), q_ptr=p(q), s_ptr=p(s), stream=st)
+        pool.expert_lists_device(n, K, E, p(sel), p(off), p(rows), p(slots), w_ptr=p(rw), w_out_ptr=p(lw), stream=st)
+        pool.grouped_matmul_device(T_E4M3, E, 2 * FF, H, n, n * K, p(q), p(wg), p(off), p(gu), T_BF16, a_scale_ptr=p(s),
+                                   w_scale_ptr=p(sg), in_rows_ptr=p(rows), stream=st)
+        pool.silu_mul_q8_device(n * K, FF, T_BF16, p(gu), q_ptr=p(hq), s_ptr=p(hs), stream=st)
+        pool.grouped_matmul_device(T_E4M3, E, H, FF, n * K, n * K, p(hq), p(wd), p(off), p(out), T_F32, a_scale_ptr=p(hs),
+                                   w_scale_ptr=p(sd), out_rows_ptr=p(slots), out_scale_ptr=p(lw), stream=st)
+
+    def fill(seed):
+        f = _gen(seed)
+        x.copy_(torch.randn(n, H, generator=f, device="cuda"))
+        res.copy_(torch.randn(n, H, generator=f, device="cuda"))
+        sel.copy_(torch.rand(n, E, generator=f, device="cuda").argsort(1)[:, :K])
+
+    fill(1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer(torch.cuda.current_stream().cuda_stream)
+    for seed in (2, 3):
+        fill(seed)
+        out.fill_(CANARY)
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [t.clone() for t in (total, s, off, slots, gu, hs, out)]
+        layer(_st())
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(replayed, (total, s, off, slots, gu, hs, out)))
+    pool.device_status(_st())
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_pool_of_another_device_than_the_current():
+    with MoePool(2048, 640, 512, 10, max_tokens=16, n_layers=1, device=1) as pool:
+        torch.cuda.set_device(0)
+        x, w = torch.ones(2, 256, device="cuda:1"), torch.ones(256, device="cuda:1")
+        y = torch.empty_like(x)
+        torch.cuda.synchronize(1)
+        pool.rmsnorm_q8_device(2, 256, T_F32, x.data_ptr(), w.data_ptr(), 0.0, y_ptr=y.data_ptr())
+        assert torch.cuda.current_device() == 0
+        pool.device_status()
+        assert bool((y == 1).all())
 
 
 @pytest.mark.parametrize("n,kind", [(1, T_E4M3), (37, T_E4M3), (37, T_BF16)])
