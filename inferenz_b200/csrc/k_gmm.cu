@@ -13,12 +13,12 @@
 // of w has one weight scale per k block, so as * ws is formed once per entry and block and kept in shared memory.
 //   warp 0      TMA producer: per 128-byte step of k a box of 128 weight rows and, unless they are gathered, the entries'
 //               rows in boxes of 16 or TN rows, 128-byte swizzle
-//   warp 1      allocates all 512 TMEM columns (4 accumulators per team), one lane issues 4 MMAs per stage
+//   warp 1      allocates all 512 TMEM columns, one lane issues 4 MMAs per step
 //   warps 2-3   stage as * ws and where each entry's result goes, ahead of the fold
 //   warps 4-7   the entries' rows by index
 //   warps 8-15  fold and write, thread = a row of w. TN = 128 (bf16 / f16): all eight warps share an item, every other 32
 //               entries; TN = 32: the two warpgroups take the items in turn, so one writes while the other folds
-// Measured on B200, top-10 of 512 experts, gate|up 1280 x 2048 e4m3: 32 tokens 79 us (6 TB/s from DRAM), one token 12.7 us;
+// Measured on B200, top-10 of 512 experts, gate|up 1280 x 2048 e4m3: 32 tokens 78 us (6 TB/s from DRAM), one token 12.2 us;
 // bf16 64 experts 1280 x 2560, 333 tokens 82 us (430 MB, 5.2 TB/s).
 // Persistent: one CTA per SM walks the items; the offsets are turned into tile numbers by every CTA for itself, which
 // costs a read of off and a scan instead of a launch. Every mbarrier wait is bounded; on expiry the CTA records an
@@ -40,16 +40,21 @@ constexpr int kGmmKc = 8;  // k blocks whose scales are staged at once
 template <int TN>
 struct GmmCfg {
     static constexpr int kTeams = TN <= 32 ? 2 : 1, kTeamWarps = 8 / kTeams;
-    static constexpr int kStages = TN <= 32 ? 10 : 6, kStage = (GM + TN) * kGmmBytes;
-    static constexpr int kAcc = 4;                              // accumulators of TN columns, per team: a team waits for its
-                                                                // own alone, so it is never two phases of one ahead
+    // A stage has kSub steps of k behind one pair of barriers, and accumulators go back in groups of kGroup: a wait on a completed
+    // barrier takes some 90 cycles, and a step of few entries, some 470 cycles, had four of them. Measured against one step and
+    // one accumulator: top-10 of 512, 1 and 2 tokens, e4m3 12.4 and 19.2 -> 12.2 and 18.1 us, 64 experts bf16 21.3 and 32.2 ->
+    // 19.2 and 31.0; a dense row, whose only item per SM waits for a whole first stage, 9.7 -> 9.7 to 10.3.
+    static constexpr int kSub = TN <= 32 ? 2 : 1, kSubBytes = (GM + TN) * kGmmBytes;
+    static constexpr int kStages = TN <= 32 ? 5 : 6, kStage = kSub * kSubBytes;
+    static constexpr int kAcc = 512 / TN / kTeams, kGroup = kAcc / 2;  // accumulators of TN columns, per team: a team
+                                                                // waits for its own alone, so it is never two phases ahead
     static constexpr int kChunks = TN / 32 / (2 / kTeams);      // 32-entry chunks per thread
 };
 
 template <int TN>
 struct GmmShared {
     using C = GmmCfg<TN>;
-    uint64_t full[C::kStages], empty[C::kStages], acc_full[C::kTeams][C::kAcc], acc_empty[C::kTeams][C::kAcc], drain;
+    uint64_t full[C::kStages], empty[C::kStages], acc_full[C::kTeams][C::kAcc], acc_empty[C::kTeams][2], drain;
     uint32_t tmem_base;
     int abort, never;
     GmmStaged<TN, C::kTeams, 1, kGmmKc> staged;
@@ -84,11 +89,10 @@ gmm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
             mbar_init(&S.full[s], A.in_rows ? 1 + kGmmGatherWarps : 1);
             mbar_init(&S.empty[s], 1);
         }
-        for (int t = 0; t < C::kTeams; t++)
-            for (int b = 0; b < NA; b++) {
-                mbar_init(&S.acc_full[t][b], 1);
-                mbar_init(&S.acc_empty[t][b], C::kTeamWarps);
-            }
+        for (int t = 0; t < C::kTeams; t++) {
+            for (int b = 0; b < NA; b++) mbar_init(&S.acc_full[t][b], 1);
+            for (int b = 0; b < 2; b++) mbar_init(&S.acc_empty[t][b], C::kTeamWarps);
+        }
         mbar_init(&S.drain, 1);
         gmm_staged_init(S.staged);
         S.abort = 0;
@@ -118,19 +122,23 @@ gmm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
                     const bool whole = I.nt > 16;
                     const uint32_t bytes = (GM + (A.in_rows ? 0 : whole ? TN : 16)) * kGmmBytes;
                     const int wrow = I.g * A.n + I.rb * GM;
-                    for (int k = 0, x = 0; k < steps; k++, x += kGmmBytes / kElem) {
+                    for (int k = 0; k < steps; k += C::kSub) {
                         if (issued == ST) {
                             if (!(ok = mbar_wait(&S.empty[slot.i], slot.parity ^ 1, abort))) break;
                         } else {
                             issued++;
                         }
-                        uint8_t *stage = ring + slot.i * C::kStage;
                         uint64_t *full = &S.full[slot.i];
-                        mbar_expect_tx(full, bytes);
-                        tma_load_2d(stage, &map_w, x, wrow, full);
-                        if (!A.in_rows) {
-                            if (whole) tma_load_2d(stage + GM * kGmmBytes, &map_a, x, I.base, full);
-                            else tma_load_2d(stage + GM * kGmmBytes, &map_a16, x, I.base, full);
+                        const int subs = min(C::kSub, steps - k);
+                        mbar_expect_tx(full, subs * bytes);
+                        for (int j = 0; j < subs; j++) {
+                            uint8_t *stage = ring + slot.i * C::kStage + j * C::kSubBytes;
+                            const int x = (k + j) * (kGmmBytes / kElem);
+                            tma_load_2d(stage, &map_w, x, wrow, full);
+                            if (!A.in_rows) {
+                                if (whole) tma_load_2d(stage + GM * kGmmBytes, &map_a, x, I.base, full);
+                                else tma_load_2d(stage + GM * kGmmBytes, &map_a16, x, I.base, full);
+                            }
                         }
                         slot.next();
                     }
@@ -151,28 +159,33 @@ gmm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
                 GmmSlot<ST> slot;
                 struct Accs {  // one team's accumulators
                     GmmSlot<NA> at;
-                    int given = 0;  // handed over, counted up to NA
+                    int given = 0;  // groups handed over, counted up to 2
                 };
                 Accs mine, other;  // of the current item's team and (two teams) of the next item's: they change places
                 const uint64_t desc0 = gmm_desc(ring);
                 for (int item = blockIdx.x, team = 0, n = 0; item < nitems && ok; item += gridDim.x, team = (team + 1) % C::kTeams, n++) {
                     const GmmItem I = gmm_item<TN>(S.walk, A, item, n);
                     const uint32_t idesc = A.idesc | (uint32_t)(((I.nt + 15) & ~15) >> 3) << 17;
-                    for (int k = 0; k < steps; k++) {
-                        const bool open = F8 || k == 0, close = F8 || k == steps - 1;
-                        if (open) {
-                            if (mine.given == NA) ok = mbar_wait(&S.acc_empty[team][mine.at.i], mine.at.parity ^ 1, abort);
-                            else mine.given++;
+                    for (int k0 = 0; k0 < steps && ok; k0 += C::kSub) {
+                        if (!(ok = mbar_wait(&S.full[slot.i], slot.parity, abort))) break;
+                        const int k1 = min(k0 + C::kSub, steps);
+                        for (int k = k0; k < k1; k++) {
+                            const bool open = F8 || k == 0, close = F8 || k == steps - 1;
+                            if (open && mine.at.i % C::kGroup == 0) {
+                                if (mine.given == 2) ok = mbar_wait(&S.acc_empty[team][mine.at.i / C::kGroup], mine.at.parity ^ 1, abort);
+                                else mine.given++;
+                                if (!ok) break;
+                            }
+                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                            const uint64_t da = desc0 + (uint64_t)((slot.i * C::kStage + (k - k0) * C::kSubBytes) >> 4);
+                            gmm_mma_stage<F8>(tmem + (team * NA + mine.at.i) * TN, da, da + (GM * kGmmBytes >> 4), idesc, open);
+                            if (close) {
+                                gmm_commit(&S.acc_full[team][mine.at.i]);
+                                mine.at.next();
+                            }
                         }
-                        if (!ok || !(ok = mbar_wait(&S.full[slot.i], slot.parity, abort))) break;
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const uint64_t da = desc0 + (uint64_t)(slot.i * (C::kStage >> 4));
-                        gmm_mma_stage<F8>(tmem + (team * NA + mine.at.i) * TN, da, da + (GM * kGmmBytes >> 4), idesc, open);
+                        if (!ok) break;
                         gmm_commit(&S.empty[slot.i]);
-                        if (close) {
-                            gmm_commit(&S.acc_full[team][mine.at.i]);
-                            mine.at.next();
-                        }
                         slot.next();
                     }
                     if constexpr (C::kTeams == 2) {
@@ -190,8 +203,8 @@ gmm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
         } else if (warp < 4) {
             if (!gmm_stage_walk<F8, TN>(S.staged, S.walk, A, nitems, abort)) S.abort = 1;
         } else if (warp >= 4) {
-            if (A.in_rows && !gmm_gather<TN, ST, kGmmGatherWarps>(S.walk, A, threadIdx.x - 128, nitems, ring, C::kStage, GM * kGmmBytes,
-                                                                  S.full, S.empty, abort))
+            if (A.in_rows && !gmm_gather<TN, ST, C::kSub, kGmmGatherWarps>(S.walk, A, threadIdx.x - 128, nitems, ring, C::kSubBytes,
+                                                                           GM * kGmmBytes, S.full, S.empty, abort))
                 S.abort = 1;
         }
     } else {
@@ -240,7 +253,7 @@ gmm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
                     }
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&S.acc_empty[team][acc.i]);
+                    if (acc.i % C::kGroup == C::kGroup - 1 && lane == 0) mbar_arrive(&S.acc_empty[team][acc.i / C::kGroup]);
                     acc.next();
                 }
                 if (!ok) break;

@@ -218,9 +218,10 @@ __device__ __forceinline__ void gmm_tmem_free(uint32_t tmem) {
 // tiled copy with 128-byte swizzle would fill, and arrive on the stage's barrier (one arrival per warp) once the copies of
 // LAG stages earlier have landed and are fenced for the tensor core's reads. tile::gather4 would need no warps, but moved
 // only four rows in some 70 ns: 225 us at 333 bf16 tokens (52 rows a tile) against 90 us with neighbouring rows.
-// Returns false when a wait ran out. tid: the thread among the gathering ones; b_off: the rows' place in a stage.
-template <int TILE, int STAGES, int WARPS>
-__device__ __forceinline__ bool gmm_gather(const GmmWalk &W, const GmmArgs &A, int tid, int nitems, uint8_t *ring, int stage_bytes,
+// Returns false when a wait ran out. tid: the thread among the gathering ones; a stage has SUB steps of sub_bytes each, b_off is the
+// rows' place in one.
+template <int TILE, int STAGES, int SUB, int WARPS>
+__device__ __forceinline__ bool gmm_gather(const GmmWalk &W, const GmmArgs &A, int tid, int nitems, uint8_t *ring, int sub_bytes,
                                            int b_off, uint64_t *full, uint64_t *empty, volatile int *abort) {
     constexpr int LAG = 2, PER = (TILE * 8 + WARPS * 32 - 1) / (WARPS * 32);  // 16-byte pieces of a stage per thread
     static_assert(LAG < STAGES && PER >= 1, "gather pipeline");
@@ -239,23 +240,27 @@ __device__ __forceinline__ bool gmm_gather(const GmmWalk &W, const GmmArgs &A, i
             // a bad index reads row 0; the fold neither writes that entry nor stays silent about it
             src[j] = A.a + ((unsigned)v < (unsigned)A.a_rows ? v : 0) * A.lda_bytes + piece * 16;
         }
-        for (int k = 0; k < A.steps; k++, kg++) {
+        for (int k = 0; k < A.steps; k += SUB, kg++) {
             const int s = kg % STAGES;
             if (kg >= STAGES) ok = mbar_wait(&empty[s], ((kg / STAGES) - 1) & 1, abort);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            const int64_t at = (int64_t)k * kGmmBytes;
-            const int64_t left = A.k_bytes - at - piece * 16;
-            const int size = left >= 16 ? 16 : left > 0 ? (int)left : 0;
-            const int64_t from = size ? at : -(int64_t)piece * 16;  // nothing is read then: stay inside the row
-            const uint32_t dst = smem_u32(ring + s * stage_bytes + b_off);
 #pragma unroll
-            for (int j = 0; j < PER; j++) {
-                const int row = row0 + j * APART;
-                if (row < n16)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + row * 128 + ((piece ^ (row & 7)) << 4)),
-                                 "l"(src[j] + from), "r"(size)
-                                 : "memory");
+            for (int u = 0; u < SUB; u++) {
+                if (SUB > 1 && k + u >= A.steps) break;
+                const int64_t at = (int64_t)(k + u) * kGmmBytes;
+                const int64_t left = A.k_bytes - at - piece * 16;
+                const int size = left >= 16 ? 16 : left > 0 ? (int)left : 0;
+                const int64_t from = size ? at : -(int64_t)piece * 16;  // nothing is read then: stay inside the row
+                const uint32_t dst = smem_u32(ring + (s * SUB + u) * sub_bytes + b_off);
+#pragma unroll
+                for (int j = 0; j < PER; j++) {
+                    const int row = row0 + j * APART;
+                    if (row < n16)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + row * 128 + ((piece ^ (row & 7)) << 4)),
+                                     "l"(src[j] + from), "r"(size)
+                                     : "memory");
+                }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
             if (kg >= LAG) {

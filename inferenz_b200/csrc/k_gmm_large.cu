@@ -195,7 +195,7 @@ gmm_large_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         } else if (warp == 2 || warp == 3) {
             if (!gmm_stage_walk<true, LM>(S.staged, S.walk, A, nitems, abort)) S.abort = 1;
         } else if (warp >= 4 && A.in_rows) {
-            if (!gmm_gather<LM, LSTAGES, kLargeGatherWarps>(S.walk, A, threadIdx.x - 128, nitems, ring, kLargeStage, 0, S.full, S.empty,
+            if (!gmm_gather<LM, LSTAGES, 1, kLargeGatherWarps>(S.walk, A, threadIdx.x - 128, nitems, ring, kLargeStage, 0, S.full, S.empty,
                                                             abort))
                 S.abort = 1;
         }
