@@ -18,7 +18,7 @@
 //   warps 4-7   the entries' rows by index
 //   warps 8-15  fold and write, thread = a row of w. TN = 128 (bf16 / f16): all eight warps share an item, every other 32
 //               entries; TN = 32: the two warpgroups take the items in turn, so one writes while the other folds
-// Measured on B200, top-10 of 512 experts, gate|up 1280 x 2048 e4m3: 32 tokens 78 us (6 TB/s from DRAM), one token 12.2 us;
+// Measured on B200, top-10 of 512 experts, gate|up 1280 x 2048 e4m3: 32 tokens 77 to 85 us (6 TB/s from DRAM), one token 11.7 us;
 // bf16 64 experts 1280 x 2560, 333 tokens 82 us (430 MB, 5.2 TB/s).
 // Persistent: one CTA per SM walks the items; the offsets are turned into tile numbers by every CTA for itself, which
 // costs a read of off and a scan instead of a launch. Every mbarrier wait is bounded; on expiry the CTA records an
@@ -26,6 +26,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "k_gmm.cuh"
 #include "k_launch.h"
@@ -84,6 +85,7 @@ gmm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
     volatile int *never = &S.never;
     constexpr int kElem = F8 ? 1 : 2;
 
+    const GmmOffsets<kGmmThreads> offsets(A);  // on their way while barriers and TMEM are set up
     if (threadIdx.x == 0) {
         for (int s = 0; s < ST; s++) {
             mbar_init(&S.full[s], A.in_rows ? 1 + kGmmGatherWarps : 1);
@@ -97,15 +99,14 @@ gmm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
         gmm_staged_init(S.staged);
         S.abort = 0;
         S.never = 0;
-        S.walk.bad = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) gmm_tmem_alloc(&S.tmem_base);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
+    __syncthreads();  // TMEM's address is read here: read after the walk it is not kept in a register (4096 tokens, down: 226 -> 235 us)
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = S.tmem_base;
-    const int nitems = gmm_walk_init<TN, kGmmThreads>(S.walk, A, blockIdx.x, gridDim.x);
+    const int nitems = gmm_walk_init<TN, kGmmThreads>(S.walk, A, offsets, blockIdx.x, gridDim.x);
     const int steps = A.steps;
 
     // registers: 128 per thread at launch, 16 warps; 8 * 88 + 8 * 168 = 16 * 128
@@ -223,46 +224,59 @@ gmm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
             float2 f[C::kChunks * 16];
 #pragma unroll
             for (int j = 0; j < C::kChunks * 16; j++) f[j] = make_float2(0.0f, 0.0f);
-            for (int b0 = 0; b0 < (F8 ? steps : 1); b0 += kGmmKc) {
-                if (F8) ok = mbar_wait(&S.staged.p_full[team][ps.i], ps.parity, abort);
-                const float(&p)[kGmmKc][TN] = S.staged.p[team][ps.i][0];
-                const int nb = F8 ? min(kGmmKc, steps - b0) : 1;
-                for (int b = 0; b < nb; b++) {
-                    if (ok) ok = mbar_wait(&S.acc_full[team][acc.i], acc.parity, abort);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            // W: columns of an accumulator that are read and factors that are fetched ahead of it. All 32 against as many as the
+            // item has, 20 steps of a dense product, us: 8 entries 10.2 -> 9.7, 24 entries as before; top-10 of 512, 4 tokens: 23.4 -> 23.2
+            auto fold = [&](auto width) {
+                constexpr int W = decltype(width)::value;
+                for (int b0 = 0; b0 < (F8 ? steps : 1); b0 += kGmmKc) {
+                    if (F8) ok = mbar_wait(&S.staged.p_full[team][ps.i], ps.parity, abort);
+                    const float(&p)[kGmmKc][TN] = S.staged.p[team][ps.i][0];
+                    const int nb = F8 ? min(kGmmKc, steps - b0) : 1;
+                    for (int b = 0; b < nb; b++) {
+                        float4 s4[W < 32 ? W / 4 : 1];
+                        if (W < 32) {
 #pragma unroll
-                    for (int c = 0; c < C::kChunks; c++) {
-                        const int c0 = (c_first + c_step * c) * 32;
-                        if (c0 >= I.nt) continue;
-                        float v[32];
-                        gmm_ld32(lanes + acc.i * TN + c_step * c * 32, v);
+                            for (int j = 0; j < W / 4; j++) s4[j] = *reinterpret_cast<const float4 *>(&p[b][j * 4]);
+                        }
+                        if (ok) ok = mbar_wait(&S.acc_full[team][acc.i], acc.parity, abort);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            const int o = c * 16 + j * 2;
-                            if (F8) {
-                                const float4 s4 = *reinterpret_cast<const float4 *>(&p[b][c0 + j * 4]);
-                                f[o] = __ffma2_rn(make_float2(v[j * 4], v[j * 4 + 1]), make_float2(s4.x, s4.y), f[o]);
-                                f[o + 1] = __ffma2_rn(make_float2(v[j * 4 + 2], v[j * 4 + 3]), make_float2(s4.z, s4.w), f[o + 1]);
-                            } else {
-                                f[o] = make_float2(v[j * 4], v[j * 4 + 1]);
-                                f[o + 1] = make_float2(v[j * 4 + 2], v[j * 4 + 3]);
+                        for (int c = 0; c < C::kChunks; c++) {
+                            const int c0 = (c_first + c_step * c) * 32;
+                            if (c0 >= I.nt) continue;
+                            float v[W];
+                            gmm_ld(lanes + acc.i * TN + c_step * c * 32, v);
+#pragma unroll
+                            for (int j = 0; j < W / 4; j++) {
+                                const int o = c * 16 + j * 2;
+                                if (F8) {
+                                    const float4 s = W < 32 ? s4[j] : *reinterpret_cast<const float4 *>(&p[b][c0 + j * 4]);
+                                    f[o] = __ffma2_rn(make_float2(v[j * 4], v[j * 4 + 1]), make_float2(s.x, s.y), f[o]);
+                                    f[o + 1] = __ffma2_rn(make_float2(v[j * 4 + 2], v[j * 4 + 3]), make_float2(s.z, s.w), f[o + 1]);
+                                } else {
+                                    f[o] = make_float2(v[j * 4], v[j * 4 + 1]);
+                                    f[o + 1] = make_float2(v[j * 4 + 2], v[j * 4 + 3]);
+                                }
                             }
                         }
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (acc.i % C::kGroup == C::kGroup - 1 && lane == 0) mbar_arrive(&S.acc_empty[team][acc.i / C::kGroup]);
+                        acc.next();
                     }
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    __syncwarp();
-                    if (acc.i % C::kGroup == C::kGroup - 1 && lane == 0) mbar_arrive(&S.acc_empty[team][acc.i / C::kGroup]);
-                    acc.next();
+                    if (!ok) break;
+                    if (F8) {
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&S.staged.p_empty[team][ps.i]);
+                        ps.next();
+                    }
                 }
-                if (!ok) break;
-                if (F8) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&S.staged.p_empty[team][ps.i]);
-                    ps.next();
-                }
-            }
+            };
+            if (F8 && TN <= 32 && I.nt <= 8) fold(std::integral_constant<int, 8>());
+            else if (F8 && TN <= 32 && I.nt <= 16) fold(std::integral_constant<int, 16>());
+            else fold(std::integral_constant<int, 32>());
             if (ok) ok = mbar_wait(&S.staged.to_full[team][ts.i], ts.parity, abort);
             ok = __all_sync(0xffffffffu, ok);
             const GmmTo(&tos)[TN] = S.staged.to[team][ts.i];

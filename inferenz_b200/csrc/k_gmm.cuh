@@ -32,7 +32,6 @@ struct alignas(16) GmmItem {
 // each group's first tile and the CTA's first items, in every CTA's shared memory
 constexpr int kGmmList = 512;
 struct GmmWalk {
-    int bad;
     int wsum[16];
     int tstart[INZG_MAX_GROUPS + 1];
     GmmItem list[kGmmList];
@@ -56,29 +55,45 @@ __device__ __forceinline__ GmmItem gmm_search(const GmmWalk &W, const GmmArgs &A
 }
 
 // the CTA's n-th item, `item` of all (n counts from 0). The search takes some 1100 cycles, an item of a short k 5000: the first
-// items are searched for side by side at the start, later ones (a CTA seldom has that many) by each role for itself.
+// items are listed at the start, later ones (a CTA seldom has that many) searched for by each role for itself.
 template <int TILE>
 __device__ __forceinline__ GmmItem gmm_item(const GmmWalk &W, const GmmArgs &A, int item, int n) {
     if (n < kGmmList) return W.list[n];
     return gmm_search<TILE>(W, A, item);
 }
 
-// Tile numbers from the offsets, by the whole block (bad set to 0 and a barrier passed before): a thread counts the tiles of
-// `per` neighbouring groups, then a scan over the block; then the CTA's items (first, first + stride, ...). Returns the number of
-// items of all CTAs, 0 when the offsets are bad. Ends with a barrier.
-template <int TILE, int THREADS>
-__device__ __forceinline__ int gmm_walk_init(GmmWalk &W, const GmmArgs &A, int item0, int stride) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int per = (A.groups + THREADS - 1) / THREADS, g0 = threadIdx.x * per, g1 = min(g0 + per, A.groups);
-    int mine = 0;
-    for (int g = g0; g < g1; g++) {
-        const int o0 = A.off ? A.off[g] : 0, o1 = A.off ? A.off[g + 1] : A.entries;
-        const bool bad = o0 < 0 || o1 < o0 || o1 > A.entries;
-        if (bad) W.bad = 1;
-        const int tiles = bad ? 0 : (o1 - o0 + TILE - 1) / TILE;
-        W.tstart[g] = mine;  // within the thread's groups so far
-        mine += tiles;
+// What a thread needs of the offsets: its groups are g0, g0 + 1, ..., their first entries o[0], o[1], ...
+template <int THREADS>
+struct GmmOffsets {
+    static constexpr int kMost = (INZG_MAX_GROUPS + THREADS - 1) / THREADS;
+    int g0, count, o[kMost + 1];
+    __device__ __forceinline__ explicit GmmOffsets(const GmmArgs &A) {
+        const int per = (A.groups + THREADS - 1) / THREADS;
+        g0 = threadIdx.x * per;
+        count = max(0, min(per, A.groups - g0));
+        o[0] = 0;
+#pragma unroll
+        for (int j = 0; j <= kMost; j++)
+            if (j <= count && count) o[j] = A.off ? __ldg(A.off + g0 + j) : j ? A.entries : 0;
     }
+};
+
+// Tile numbers from the offsets, by the whole block: a thread counts the tiles of its groups, a scan over the block numbers them,
+// and the thread enters those of its items that are the CTA's (first, first + stride, ...) in the CTA's list. Returns the number of
+// items of all CTAs, 0 when the offsets are bad. Against a search for each of the CTA's items after the scan, and with the offsets
+// on their way during the setup, 1 token of top-10 of 512 takes 11.5 us instead of 12.2. What the block's threads wrote to shared memory before is seen by all afterwards.
+template <int TILE, int THREADS>
+__device__ __forceinline__ int gmm_walk_init(GmmWalk &W, const GmmArgs &A, const GmmOffsets<THREADS> &O, int first, int stride) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto tiles_of = [&](int j) { return (O.o[j + 1] - O.o[j] + TILE - 1) / TILE; };
+    bool bad = false;
+    int mine = 0;
+#pragma unroll
+    for (int j = 0; j < O.kMost; j++)
+        if (j < O.count) {
+            if (O.o[j] < 0 || O.o[j + 1] < O.o[j] || O.o[j + 1] > A.entries) bad = true;
+            else mine += tiles_of(j);
+        }
     int scan = mine;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
@@ -86,21 +101,45 @@ __device__ __forceinline__ int gmm_walk_init(GmmWalk &W, const GmmArgs &A, int i
         if (lane >= d) scan += v;
     }
     if (lane == 31) W.wsum[warp] = scan;
-    __syncthreads();
-    int first = scan - mine;
-    for (int k = 0; k < warp; k++) first += W.wsum[k];
-    for (int g = g0; g < g1; g++) W.tstart[g] += first;
-    if (g0 < A.groups && g1 == A.groups) W.tstart[A.groups] = first + mine;
-    __syncthreads();
-    if (W.bad) {
+    if (__syncthreads_or(bad)) {
         if (threadIdx.x == 0) atomicCAS(A.err, kErrNone, kErrOverflow);
         return 0;
     }
-    const int nitems = W.tstart[A.groups] * A.nrb;
-    for (int n = threadIdx.x; n < kGmmList && item0 + (int64_t)n * stride < nitems; n += THREADS)
-        W.list[n] = gmm_search<TILE>(W, A, item0 + n * stride);
+    int at = scan - mine, all = 0;
+#pragma unroll
+    for (int k = 0; k < THREADS / 32; k++) {
+        const int v = W.wsum[k];
+        if (k < warp) at += v;
+        all += v;
+    }
+    if (threadIdx.x == 0) W.tstart[A.groups] = all;
+    const int dt = stride / A.nrb, dr = stride - dt * A.nrb;
+#pragma unroll
+    for (int j = 0; j < O.kMost; j++)
+        if (j < O.count) {
+            const int tiles = tiles_of(j), lo = at * A.nrb;
+            W.tstart[O.g0 + j] = at;
+            if (tiles) {
+                int n = lo > first ? (lo - first + stride - 1) / stride : 0;
+                const int skip = first + n * stride - lo;
+                int t = skip / A.nrb, rb = skip - t * A.nrb;
+                for (; t < tiles && n < kGmmList; n++, t += dt, rb += dr) {
+                    if (rb >= A.nrb) {
+                        rb -= A.nrb;
+                        if (++t >= tiles) break;
+                    }
+                    GmmItem I;
+                    I.g = O.g0 + j;
+                    I.base = O.o[j] + t * TILE;
+                    I.nt = min(TILE, O.o[j + 1] - I.base);
+                    I.rb = rb;
+                    W.list[n] = I;
+                }
+            }
+            at += tiles;
+        }
     __syncthreads();
-    return nitems;
+    return all * A.nrb;
 }
 
 // One lane of a converged warp. The producer and the MMA warp run their whole loops under this predicate: the compiler then
@@ -158,8 +197,8 @@ __device__ __forceinline__ void gmm_commit(uint64_t *bar) {
                  : "memory");
 }
 
-// 32 columns of the warp's 32 TMEM lanes
-__device__ __forceinline__ void gmm_ld32(uint32_t taddr, float (&v)[32]) {
+// as many columns of the warp's 32 TMEM lanes as v has places
+__device__ __forceinline__ void gmm_ld(uint32_t taddr, float (&v)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
         "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
@@ -168,6 +207,25 @@ __device__ __forceinline__ void gmm_ld32(uint32_t taddr, float (&v)[32]) {
           "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
           "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
           "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(taddr)
+        : "memory");
+}
+
+__device__ __forceinline__ void gmm_ld(uint32_t taddr, float (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+          "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
+
+__device__ __forceinline__ void gmm_ld(uint32_t taddr, float (&v)[8]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
         : "r"(taddr)
         : "memory");
 }
