@@ -18,7 +18,7 @@
 //   warps 4-7   the entries' rows by index
 //   warps 8-15  fold and write, thread = a row of w. TN = 128 (bf16 / f16): all eight warps share an item, every other 32
 //               entries; TN = 32: the two warpgroups take the items in turn, so one writes while the other folds
-// Measured on B200, top-10 of 512 experts, gate|up 1280 x 2048 e4m3: 32 tokens 77 to 85 us (6 TB/s from DRAM), one token 11.7 us;
+// Measured on B200, top-10 of 512 experts, gate|up 1280 x 2048 e4m3: 32 tokens 77 to 85 us (6 TB/s from DRAM), one token 11.5 us;
 // bf16 64 experts 1280 x 2560, 333 tokens 82 us (430 MB, 5.2 TB/s).
 // Persistent: one CTA per SM walks the items; the offsets are turned into tile numbers by every CTA for itself, which
 // costs a read of off and a scan instead of a launch. Every mbarrier wait is bounded; on expiry the CTA records an
@@ -41,14 +41,16 @@ constexpr int kGmmKc = 8;  // k blocks whose scales are staged at once
 template <int TN>
 struct GmmCfg {
     static constexpr int kTeams = TN <= 32 ? 2 : 1, kTeamWarps = 8 / kTeams;
-    // A stage has kSub steps of k behind one pair of barriers, and accumulators go back in groups of kGroup: a wait on a completed
-    // barrier takes some 90 cycles, and a step of few entries, some 470 cycles, had four of them. Measured against one step and
-    // one accumulator: top-10 of 512, 1 and 2 tokens, e4m3 12.4 and 19.2 -> 12.2 and 18.1 us, 64 experts bf16 21.3 and 32.2 ->
-    // 19.2 and 31.0; a dense row, whose only item per SM waits for a whole first stage, 9.7 -> 9.7 to 10.3.
+    // A stage has kSub steps of k behind one pair of barriers; of e4m3 they are handed to the fold together (a slot of kSub
+    // accumulators) and slots go back in groups of kGroup: a wait on a completed barrier takes some 90 cycles, and a step of few
+    // entries, some 470 cycles, had four of them. Measured against one step and one accumulator at a time, us: a dense row of
+    // 10240 x 2560 9.7 -> 9.0, top-10 of 512 e4m3, 2 tokens 17.9 -> 16.5, 64 experts bf16, 2 tokens 32.2 -> 28.0. A step of one
+    // item alone now takes some 320 cycles in both types, 18 KB at 57 bytes a cycle: what one SM gets from L2.
     static constexpr int kSub = TN <= 32 ? 2 : 1, kSubBytes = (GM + TN) * kGmmBytes;
     static constexpr int kStages = TN <= 32 ? 5 : 6, kStage = kSub * kSubBytes;
-    static constexpr int kAcc = 512 / TN / kTeams, kGroup = kAcc / 2;  // accumulators of TN columns, per team: a team
-                                                                // waits for its own alone, so it is never two phases ahead
+    static constexpr int kSlot = kSub * TN;                     // TMEM columns of a slot
+    static constexpr int kAcc = 512 / kSlot / kTeams, kGroup = kAcc / 2;  // slots per team: a team waits for its own alone, so it
+                                                                // is never two phases ahead
     static constexpr int kChunks = TN / 32 / (2 / kTeams);      // 32-entry chunks per thread
 };
 
@@ -130,7 +132,7 @@ gmm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
                             issued++;
                         }
                         uint64_t *full = &S.full[slot.i];
-                        const int subs = min(C::kSub, steps - k);
+                        const int subs = C::kSub == 1 ? 1 : min(C::kSub, steps - k);
                         mbar_expect_tx(full, subs * bytes);
                         for (int j = 0; j < subs; j++) {
                             uint8_t *stage = ring + slot.i * C::kStage + j * C::kSubBytes;
@@ -167,25 +169,25 @@ gmm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
                 for (int item = blockIdx.x, team = 0, n = 0; item < nitems && ok; item += gridDim.x, team = (team + 1) % C::kTeams, n++) {
                     const GmmItem I = gmm_item<TN>(S.walk, A, item, n);
                     const uint32_t idesc = A.idesc | (uint32_t)(((I.nt + 15) & ~15) >> 3) << 17;
-                    for (int k0 = 0; k0 < steps && ok; k0 += C::kSub) {
+                    for (int k0 = 0; k0 < steps; k0 += C::kSub) {
                         if (!(ok = mbar_wait(&S.full[slot.i], slot.parity, abort))) break;
-                        const int k1 = min(k0 + C::kSub, steps);
-                        for (int k = k0; k < k1; k++) {
-                            const bool open = F8 || k == 0, close = F8 || k == steps - 1;
-                            if (open && mine.at.i % C::kGroup == 0) {
-                                if (mine.given == 2) ok = mbar_wait(&S.acc_empty[team][mine.at.i / C::kGroup], mine.at.parity ^ 1, abort);
-                                else mine.given++;
-                                if (!ok) break;
-                            }
-                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                            const uint64_t da = desc0 + (uint64_t)((slot.i * C::kStage + (k - k0) * C::kSubBytes) >> 4);
-                            gmm_mma_stage<F8>(tmem + (team * NA + mine.at.i) * TN, da, da + (GM * kGmmBytes >> 4), idesc, open);
-                            if (close) {
-                                gmm_commit(&S.acc_full[team][mine.at.i]);
-                                mine.at.next();
-                            }
+                        const int subs = C::kSub == 1 ? 1 : min(C::kSub, steps - k0);
+                        const bool open = F8 || k0 == 0, close = F8 || k0 + C::kSub >= steps;
+                        if (open && mine.at.i % C::kGroup == 0) {
+                            if (mine.given == 2) ok = mbar_wait(&S.acc_empty[team][mine.at.i / C::kGroup], mine.at.parity ^ 1, abort);
+                            else mine.given++;
+                            if (!ok) break;
                         }
-                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        for (int j = 0; j < subs; j++) {
+                            const uint64_t da = desc0 + (uint64_t)((slot.i * C::kStage + j * C::kSubBytes) >> 4);
+                            gmm_mma_stage<F8>(tmem + (team * NA + mine.at.i) * C::kSlot + (F8 ? j * TN : 0), da,
+                                              da + (GM * kGmmBytes >> 4), idesc, F8 || k0 + j == 0);
+                        }
+                        if (close) {
+                            gmm_commit(&S.acc_full[team][mine.at.i]);
+                            mine.at.next();
+                        }
                         gmm_commit(&S.empty[slot.i]);
                         slot.next();
                     }
@@ -218,7 +220,7 @@ gmm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
         bool ok = true;
         GmmSlot<NA> acc;
         GmmSlot<kGmmRing> ps, ts;
-        const uint32_t lanes = tmem + ((uint32_t)(sub * 32) << 16) + team * NA * TN + c_first * 32;
+        const uint32_t lanes = tmem + ((uint32_t)(sub * 32) << 16) + team * NA * C::kSlot + c_first * 32;
         for (int item = blockIdx.x + team * gridDim.x, n = team; item < nitems && ok; item += C::kTeams * gridDim.x, n += C::kTeams) {
             const GmmItem I = gmm_item<TN>(S.walk, A, item, n);
             float2 f[C::kChunks * 16];
@@ -232,32 +234,54 @@ gmm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
                     if (F8) ok = mbar_wait(&S.staged.p_full[team][ps.i], ps.parity, abort);
                     const float(&p)[kGmmKc][TN] = S.staged.p[team][ps.i][0];
                     const int nb = F8 ? min(kGmmKc, steps - b0) : 1;
-                    for (int b = 0; b < nb; b++) {
-                        float4 s4[W < 32 ? W / 4 : 1];
-                        if (W < 32) {
+                    for (int b = 0; b < nb; b += F8 ? C::kSub : 1) {
+                        const uint32_t from = lanes + acc.i * C::kSlot;
+                        const bool two = F8 && b + 1 < nb;
+                        float4 s4[2][W < 32 ? W / 4 : 1];
+                        if constexpr (W < 32) {
 #pragma unroll
-                            for (int j = 0; j < W / 4; j++) s4[j] = *reinterpret_cast<const float4 *>(&p[b][j * 4]);
+                            for (int q = 0; q < 2; q++)
+#pragma unroll
+                                for (int j = 0; j < W / 4; j++)
+                                    s4[q][j] = q == 0 || two ? *reinterpret_cast<const float4 *>(&p[b + q][j * 4]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                         }
                         if (ok) ok = mbar_wait(&S.acc_full[team][acc.i], acc.parity, abort);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        auto add = [&](float2 *to, const float *v, const float4 &s) {
+                            to[0] = __ffma2_rn(make_float2(v[0], v[1]), make_float2(s.x, s.y), to[0]);
+                            to[1] = __ffma2_rn(make_float2(v[2], v[3]), make_float2(s.z, s.w), to[1]);
+                        };
+                        if constexpr (W < 32) {
+                            float v[2][W];
+                            gmm_ld(from, two ? from + TN : from, v);
 #pragma unroll
-                        for (int c = 0; c < C::kChunks; c++) {
-                            const int c0 = (c_first + c_step * c) * 32;
-                            if (c0 >= I.nt) continue;
-                            float v[W];
-                            gmm_ld(lanes + acc.i * TN + c_step * c * 32, v);
+                            for (int q = 0; q < 2; q++)
+                                if (q == 0 || two) {
 #pragma unroll
-                            for (int j = 0; j < W / 4; j++) {
-                                const int o = c * 16 + j * 2;
-                                if (F8) {
-                                    const float4 s = W < 32 ? s4[j] : *reinterpret_cast<const float4 *>(&p[b][c0 + j * 4]);
-                                    f[o] = __ffma2_rn(make_float2(v[j * 4], v[j * 4 + 1]), make_float2(s.x, s.y), f[o]);
-                                    f[o + 1] = __ffma2_rn(make_float2(v[j * 4 + 2], v[j * 4 + 3]), make_float2(s.z, s.w), f[o + 1]);
-                                } else {
-                                    f[o] = make_float2(v[j * 4], v[j * 4 + 1]);
-                                    f[o + 1] = make_float2(v[j * 4 + 2], v[j * 4 + 3]);
+                                    for (int j = 0; j < W / 4; j++) add(&f[j * 2], &v[q][j * 4], s4[q][j]);
+                                }
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < C::kChunks; c++) {
+                                const int c0 = (c_first + c_step * c) * 32;
+                                if (c0 >= I.nt) continue;
+#pragma unroll
+                                for (int q = 0; q < (F8 ? C::kSub : 1); q++) {
+                                    if (q && !two) break;
+                                    float v[32];
+                                    gmm_ld(from + q * TN + c_step * c * 32, v);
+#pragma unroll
+                                    for (int j = 0; j < 8; j++) {
+                                        float2 *to = &f[c * 16 + j * 2];
+                                        if (F8) {
+                                            add(to, &v[j * 4], *reinterpret_cast<const float4 *>(&p[b + q][c0 + j * 4]));
+                                        } else {
+                                            to[0] = make_float2(v[j * 4], v[j * 4 + 1]);
+                                            to[1] = make_float2(v[j * 4 + 2], v[j * 4 + 3]);
+                                        }
+                                    }
                                 }
                             }
                         }

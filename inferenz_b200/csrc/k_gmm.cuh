@@ -211,22 +211,26 @@ __device__ __forceinline__ void gmm_ld(uint32_t taddr, float (&v)[32]) {
         : "memory");
 }
 
-__device__ __forceinline__ void gmm_ld(uint32_t taddr, float (&v)[16]) {
+// the first columns of two accumulators
+__device__ __forceinline__ void gmm_ld(uint32_t first, uint32_t second, float (&v)[2][8]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%16];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%17];\n\t"
         "tcgen05.wait::ld.sync.aligned;"
-        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
-          "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
-        : "r"(taddr)
+        : "=f"(v[0][0]), "=f"(v[0][1]), "=f"(v[0][2]), "=f"(v[0][3]), "=f"(v[0][4]), "=f"(v[0][5]), "=f"(v[0][6]), "=f"(v[0][7]),
+          "=f"(v[1][0]), "=f"(v[1][1]), "=f"(v[1][2]), "=f"(v[1][3]), "=f"(v[1][4]), "=f"(v[1][5]), "=f"(v[1][6]), "=f"(v[1][7])
+        : "r"(first), "r"(second)
         : "memory");
 }
 
-__device__ __forceinline__ void gmm_ld(uint32_t taddr, float (&v)[8]) {
+__device__ __forceinline__ void gmm_ld(uint32_t first, uint32_t second, float (&v)[2][16]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n\t"
         "tcgen05.wait::ld.sync.aligned;"
-        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
-        : "r"(taddr)
+        : "=f"(v[0][0]), "=f"(v[0][1]), "=f"(v[0][2]), "=f"(v[0][3]), "=f"(v[0][4]), "=f"(v[0][5]), "=f"(v[0][6]), "=f"(v[0][7]), "=f"(v[0][8]), "=f"(v[0][9]), "=f"(v[0][10]), "=f"(v[0][11]), "=f"(v[0][12]), "=f"(v[0][13]), "=f"(v[0][14]), "=f"(v[0][15]),
+          "=f"(v[1][0]), "=f"(v[1][1]), "=f"(v[1][2]), "=f"(v[1][3]), "=f"(v[1][4]), "=f"(v[1][5]), "=f"(v[1][6]), "=f"(v[1][7]), "=f"(v[1][8]), "=f"(v[1][9]), "=f"(v[1][10]), "=f"(v[1][11]), "=f"(v[1][12]), "=f"(v[1][13]), "=f"(v[1][14]), "=f"(v[1][15])
+        : "r"(first), "r"(second)
         : "memory");
 }
 
