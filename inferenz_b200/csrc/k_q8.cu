@@ -7,7 +7,7 @@
 // Both read each input once and write each output once: the row stays in registers (fp32) between the sum of squares
 // and the outputs, the block's largest value is a shuffle over 16 lanes, nothing passes through memory in between.
 // Measured on B200: norm of 4096 x 2560 bf16 with residual, y and e4m3 19.9 us (94.7 MB, 4.75 TB/s; 24.7 us without the next
-// row's loads in flight), one row 2.8 us; SiLU of 40960 x 640 bf16 33 us (131.9 MB, 4.0 TB/s; bound by instruction issue).
+// row's loads in flight), one row 2.8 us; SiLU of 40960 x 640 bf16 26.1 to 26.9 us (131.9 MB, 5 TB/s).
 #include "k_launch.h"
 #include "k_q8.cuh"
 
@@ -94,25 +94,30 @@ __global__ void __launch_bounds__(NCH > 2 ? 1024 : 512) rmsnorm_q8_kernel(const 
     }
 }
 
-// exp(x) for |x| <= 88, x clamped to that: 2^(x log2 e) with the product's rounding error carried to first order, so that the
-// relative error stays at a few 2^-24 for large |x| too, where the hardware's 2^t on the rounded product alone loses |x| * 2^-24.
-__device__ __forceinline__ float exp_carried(float x) {
-    x = fminf(fmaxf(x, -88.0f), 88.0f);
-    const float t = x * 1.4426950408889634f;
-    const float lo = fmaf(x, 1.925963033500938e-8f, fmaf(x, 1.4426950408889634f, -t));  // log2 e = hi + 1.926e-8
-    float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-    return fmaf(e, lo * 0.6931471805599453f, e);
+// g / (1 + exp(-g)) of two values, in packed arithmetic. With x = g clamped to 88 and t = x log2 e rounded, exp(-x) =
+// 2^-t exp(t ln 2 - x); the last factor is within 2^-17 of 1, so 1 + (t ln 2 - x) stands for it and the relative error stays at a few
+// 2^-24 for large |x| too, where 2^-t alone loses |x| * 2^-24. Below -87.3 the divisor passes 2^126 and its estimated reciprocal
+// is 0 (and the quotient NaN for -infinity); the true value is less than 2^-119 there. A NaN passes through the last product.
+__device__ __forceinline__ float2 silu2(float2 g) {
+    const float2 x = make_float2(fminf(fmaxf(g.x, -88.0f), 88.0f), fminf(fmaxf(g.y, -88.0f), 88.0f));
+    const float2 t = __fmul2_rn(x, make_float2(1.4426950408889634f, 1.4426950408889634f));
+    const float hi = 0.69314718246459961f, lo = -1.9046542999848e-9f;  // ln 2 = hi + lo
+    const float2 r = __ffma2_rn(t, make_float2(-hi, -hi), x);          // x - t hi
+    const float2 c = __ffma2_rn(t, make_float2(lo, lo), make_float2(1.0f, 1.0f));
+    const float2 m = __ffma2_rn(r, make_float2(-1.0f, -1.0f), c);  // 1 + t ln 2 - x
+    float2 e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(-t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(-t.y));
+    const float2 d = __ffma2_rn(e, m, make_float2(1.0f, 1.0f));
+    return __fmul2_rn(g, make_float2(rcp_approx(d.x), rcp_approx(d.y)));
 }
 
-// g / (1 + exp(-g)). Below -87.3 the divisor passes 2^126 and the fast division gives 0 (or NaN for -infinity); the true value is
-// less than 2^-119 there. A NaN passes through the product.
-__device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.0f + exp_carried(-g)); }
-
 // A thread's slot: one chunk of one row; slots per row are rounded up to whole blocks of 128 columns. A thread goes on by
-// `step_rows` rows and `step_chunks` chunks, the grid's size in slots, and has the next slot's loads in flight.
+// `step_rows` rows and `step_chunks` chunks, the grid's size in slots, and has the next slot's loads in flight. Four blocks per SM
+// (64 registers): 40960 x 640 bf16 26.1 us; 2 blocks 35.9, 3 28.8, 5 27.4, 6 28.0, 8 27.8; four with two slots ahead 29.1.
+constexpr int kSiluBlocks = 4;
 template <class T, bool VEC>
-__global__ void __launch_bounds__(256) silu_mul_q8_kernel(const inzg_silu_mul_q8_args A, uint32_t slots, uint32_t per_row,
+__global__ void __launch_bounds__(256, kSiluBlocks) silu_mul_q8_kernel(const inzg_silu_mul_q8_args A, uint32_t slots, uint32_t per_row,
                                                           uint32_t step_rows, uint32_t step_chunks) {
     const int cols = A.cols;
     uint32_t i = blockIdx.x * blockDim.x + threadIdx.x, row = i / per_row, chunk = i % per_row;
@@ -144,7 +149,11 @@ __global__ void __launch_bounds__(256) silu_mul_q8_kernel(const inzg_silu_mul_q8
         }
         load();
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] *= silu(gate[j]);
+        for (int j = 0; j < 8; j += 2) {
+            const float2 o = __fmul2_rn(silu2(make_float2(gate[j], gate[j + 1])), make_float2(v[j], v[j + 1]));
+            v[j] = o.x;
+            v[j + 1] = o.y;
+        }
         if (A.y && left > 0) store_chunk<T, VEC>(static_cast<T *>(A.y) + r * A.ldy + c, left, v);
         if (A.q) {
             float s;
@@ -214,7 +223,7 @@ static int silu_typed(inzg_silu_mul_q8_args A, int num_sms, cudaStream_t st) {
         if (A.q) P.q = static_cast<uint8_t *>(A.q) + done * A.ldq;
         if (A.s) P.s = A.s + done * A.lds;
         const uint32_t slots = (uint32_t)P.n * per_row;
-        const uint32_t want = (slots + 255) / 256, most = (uint32_t)num_sms * 6;
+        const uint32_t want = (slots + 255) / 256, most = (uint32_t)num_sms * kSiluBlocks;
         const uint32_t grid = want < most ? want : most, step = grid * 256;
         if (vec) silu_mul_q8_kernel<T, true><<<grid, 256, 0, st>>>(P, slots, per_row, step / per_row, step % per_row);
         else silu_mul_q8_kernel<T, false><<<grid, 256, 0, st>>>(P, slots, per_row, step / per_row, step % per_row);

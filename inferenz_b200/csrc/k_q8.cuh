@@ -119,9 +119,13 @@ __device__ __forceinline__ float rcp_approx(float x) {
 
 // 8 products as e4m3
 __device__ __forceinline__ uint2 e4m3_times(const float (&v)[8], float f) {
-    uint2 q;
-    q.x = cvt_e4m3x2(v[0] * f, v[1] * f) | cvt_e4m3x2(v[2] * f, v[3] * f) << 16;
-    q.y = cvt_e4m3x2(v[4] * f, v[5] * f) | cvt_e4m3x2(v[6] * f, v[7] * f) << 16;
+    uint32_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 o = __fmul2_rn(make_float2(v[2 * i], v[2 * i + 1]), make_float2(f, f));
+        h[i] = cvt_e4m3x2(o.x, o.y);
+    }
+    const uint2 q = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
     return q;
 }
 

@@ -4,8 +4,8 @@ Tolerances, with u = 2^-24 (half an fp32 step) and e = finfo(type).eps / 2 (one 
 * norm: h is one rounding of x + res; the sum of squares adds at most 32 squares per thread and ten shuffles, each
   rounding once, all terms positive: relative 43u, half of that in r; the mean's division, eps, the square root, the
   reciprocal and two products add 6u, h itself 2u (once in the product, once in r): 30u, then e.
-* silu: exp(-g) within 4u (the product's error carried, 2^t good to 2 ulp), 1 + exp 1u, the fast quotient 4u, the product
-  1u; where exp(-g) leaves the normal range (g < -87) or the quotient's divisor passes 2^126 the value may be 0 while
+* silu: exp(-g) within 6u (2^t good to 2 ulp, the factor that carries the product's error 2u), 1 + exp 1u, the reciprocal 2u,
+  two products 1u each; where exp(-g) leaves the normal range (g < -87) or the quotient's divisor passes 2^126 the value may be 0 while
   the true one is below 2^-120 |u|.
 * scales: one rounding more than the values' largest; q: half a step of e4m3 at v / s (2^-4 relative, 2^-10 below the
   smallest normal) plus the value's own error, 4u for the scale and its reciprocal.
