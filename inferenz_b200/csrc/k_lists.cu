@@ -1,13 +1,14 @@
 // k_lists.cu -- the entries of the router's selections in order of expert, on sm_100a (inzg_expert_lists): a stable counting sort
 // without scratch in global memory; its shared-memory atomics only count and set bits, so the order is fixed.
 //
-// One block, or for more than 2048 entries a cluster of eight. A warp owns a contiguous run of the entries, a row of
+// One block, or for more than 2048 entries a cluster of sixteen (past the portable eight, which took 14.1 us
+// where this takes 11.7: the scattered results leave through twice the SMs). A warp owns a contiguous run of the entries, a row of
 // counters in shared memory, one per expert, and a row of lane masks: within a step of 32 entries the lanes set their bits in
 // their experts' masks (match.any, which does the same, goes through the distinct values one by one and was slower), so that
 //   place = (entries of smaller experts) + (own expert: earlier blocks, earlier warps, earlier steps, lower lanes)
 // The blocks of the cluster read one another's totals through distributed shared memory. Each entry is read twice; what bounds it
 // is the chain of two passes, a scan over the experts and two cluster barriers. A block per expert (or per four) that counted
-// every entry for itself took 20 to 26 us at 4096 tokens, top-10; this takes 14.1 us, and 3.6 us at 32 tokens.
+// every entry for itself took 20 to 26 us at 4096 tokens, top-10; this takes 11.7 us, and 3.6 us at 32 tokens.
 #include <algorithm>
 
 #include "inzg_internal.h"
@@ -16,7 +17,7 @@
 
 namespace inzg {
 
-constexpr int kListThreads = 1024, kListCluster = 8, kListCounters = 24576;  // counters of all warps, and as many masks: 192 KB
+constexpr int kListThreads = 1024, kListCluster = 16, kListCounters = 24576;  // counters of all warps, and as many masks: 192 KB
 
 __device__ __forceinline__ void lists_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -141,6 +142,7 @@ void lists_set_attributes() {
     const int most = (2 * kListCounters + 2 * INZG_MAX_GROUPS) * (int)sizeof(int);
     cudaFuncSetAttribute(expert_lists_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     cudaFuncSetAttribute(expert_lists_kernel<kListCluster>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    cudaFuncSetAttribute(expert_lists_kernel<kListCluster>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
 }
 
 int launch_expert_lists(int n, int topk, int E, const int32_t *sel, const float *w, int32_t *off, int32_t *rows,
