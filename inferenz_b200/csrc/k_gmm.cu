@@ -413,18 +413,22 @@ int launch_grouped_matmul(const inzg_grouped_matmul_args &G, int num_sms, int32_
     // fp32 accumulators; e4m3 (0), bf16 (1) or f16 (0) operands, both K-major; M = 128
     const uint32_t fmt = G.type == INZG_T_BF16 ? 1u : 0u;
     A.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(GM >> 4) << 24);
-    // Which kernel, by the entries per group (measured at k = 2048 and 2560 with 1280 columns, us):
-    //   bf16, 64 groups:    20 a group: 32-entry tiles 76, 128-entry tiles 81; 30 a group: 88, 81; 160 a group: 265, 121
-    //   e4m3, 64 groups:    40 a group: 32-entry tiles 47, 128 x 256 tiles 53; 62 a group: 61, 53; 160 a group: 124, 67
-    //   e4m3, 8 groups:     64 a group: 32-entry tiles 15, 128 x 256 tiles 20; 128 a group: 21, 20
-    // The last case has fewer large tiles than half the SMs, and small ones fill the GPU better.
+    // Which kernel, by the entries per group and by how many 32-entry items there are, taken to be one per 32 entries and half a one
+    // more per group (measured with k = 2048 and 2560, 32-entry tiles against 128-entry ones, us):
+    //   e4m3, 64 groups, n = 1280: 50 a group 44, 52; 62: 52, 53; 69: 55, 53; 80: 58, 52
+    //   e4m3, 512 groups, n = 640: 50 a group 150, 173; 62: 180, 190; 70: 192, 190
+    //   e4m3, one group, n = 2560: 128 entries 9.8, 16.5; 448: 14.4, 17.2; n = 10240: 96 entries 15.3, 17.2; 128: 18.8, 17.7
+    //   bf16, 64 groups, n = 1280: 40 a group 75, 82; 45: 80, 82; 52: 85, 81
+    //   bf16, one group, n = 1280: 192 entries 13, 19; n = 40960: 32 entries 42, 53; 64: 71, 57
+    // The entries of one group alone fill their tiles: past 32 its bf16 weights are streamed twice. A few items, up to one per SM
+    // (e4m3: two), are sooner done in small tiles whatever the groups.
+    const int64_t few = std::min<int64_t>(G.entries, (G.entries + 31LL) / 32 + (G.groups - 1) / 2) * A.nrb;
     if (G.type != INZG_T_E4M3) {
-        if (G.entries <= 24 * (int64_t)G.groups || !g_wide_ok) return gmm_launch<false, 32>(G, A, num_sms, st);
+        if (G.entries <= (G.groups > 1 ? 40 : 32) * (int64_t)G.groups || few <= num_sms || !g_wide_ok)
+            return gmm_launch<false, 32>(G, A, num_sms, st);
         return gmm_launch<false, 128>(G, A, num_sms, st);
     }
-    const int64_t large_items = std::min<int64_t>(G.entries, G.entries / 128 + G.groups) * ((G.n + 255) / 256);
-    if (G.entries <= (large_items <= num_sms / 2 ? 96 : 48) * (int64_t)G.groups || !g_large_ok)
-        return gmm_launch<true, 32>(G, A, num_sms, st);
+    if (G.entries <= 64 * (int64_t)G.groups || few <= 2 * num_sms || !g_large_ok) return gmm_launch<true, 32>(G, A, num_sms, st);
     return gmm_large_launch(G, A, num_sms, st);
 }
 

@@ -330,7 +330,8 @@ def _product_bound(absprod, k, f8, exact, dt):
 
 MATMUL = [(1, 1, 1), (1, 640, 2560), (2, 127, 16), (3, 128, 64), (15, 129, 127), (16, 130, 128), (17, 257, 129),
           (33, 16, 640), (63, 64, 1040), (64, 128, 2048), (65, 300, 256), (96, 129, 1000), (127, 128, 1153), (128, 384, 512),
-          (129, 1, 300), (300, 260, 2064), (1000, 70, 96), (5, 2000, 48), (257, 1300, 700)]
+          (129, 1, 300), (300, 260, 2064), (1000, 70, 96), (5, 2000, 48), (257, 1300, 700),
+          (9700, 70, 96), (1000, 1300, 700), (257, 5000, 300), (129, 8000, 1153), (2500, 512, 2064)]  # more tiles than two per SM
 
 
 @pytest.mark.parametrize("m,n,k", MATMUL)
@@ -352,7 +353,7 @@ def test_matmul_exact(pool, m, n, k, out):
 
 
 @pytest.mark.parametrize("m,n,k,out", [(1, 1280, 2560, T_BF16), (77, 300, 1111, T_F32), (400, 640, 2048, T_F16),
-                                       (130, 2560, 640, T_F32)])
+                                       (130, 2560, 640, T_F32), (1000, 1300, 2048, T_BF16)])
 def test_matmul_real(pool, m, n, k, out):
     g, kb = _gen(m), (k + 127) // 128
     fp8 = lambda r: (torch.randn(r, _up(k, 16), generator=g, device="cuda") * 120).clamp(-448, 448).to(F8)[:, :k]  # noqa: E731
@@ -442,7 +443,8 @@ def _grouped_want(c, E, entries, n):
 
 
 GROUPED = [(1, 1, 128, 128), (1, 200, 130, 160), (4, 3, 64, 1), (8, 40, 256, 640), (16, 10, 1280, 2048), (5, 333, 127, 129),
-           (64, 500, 129, 320), (512, 320, 128, 256), (2, 700, 260, 96), (2048, 100, 16, 32), (3, 129, 1, 2048)]
+           (64, 500, 129, 320), (512, 320, 128, 256), (2, 700, 260, 96), (2048, 100, 16, 32), (3, 129, 1, 2048),
+           (1, 10_300, 127, 129), (16, 9000, 130, 2064), (100, 7000, 260, 300), (3, 1700, 1300, 520), (2, 640, 2000, 20_011)]
 
 
 @pytest.mark.parametrize("E,entries,n,k", GROUPED)
@@ -460,7 +462,8 @@ def test_grouped_exact(pool, E, entries, n, k, t, out, gather, scatter):
 
 
 @pytest.mark.parametrize("t", [T_E4M3, T_BF16, T_F16])
-@pytest.mark.parametrize("E,entries,n,k,out", [(16, 10, 1280, 2048, T_F32), (6, 450, 640, 1100, T_BF16), (3, 700, 200, 520, T_F32)])
+@pytest.mark.parametrize("E,entries,n,k,out", [(16, 10, 1280, 2048, T_F32), (6, 450, 640, 1100, T_BF16), (3, 700, 200, 520, T_F32),
+                                             (100, 7000, 260, 1100, T_BF16)])
 def test_grouped_real(pool, t, E, entries, n, k, out):
     c = _grouped_case(t, E, entries, n, k, True, True, 5 + E, ints=False)
     o, _ = _run_grouped(pool, t, c, E, entries, n, k, out)
@@ -542,6 +545,73 @@ def test_grouped_checks_on_the_device(pool, break_it, word):
     else:
         want[good["to"][bad_entry].long()] = CANARY
         assert torch.equal(o.double(), want)
+    pool.device_status(_st())
+
+
+@pytest.mark.parametrize("t", [T_E4M3, T_BF16])
+def test_many_entries_checked_partial_and_replayed(pool, t):
+    """the tiles of many entries: bad offsets and indexes, lists that leave entries out, no listed entries, NaN in one row, a
+    replay on new contents"""
+    E, entries, n, k = 100, 7000, 400, 256
+    base = _grouped_case(t, E, entries, n, k, True, True, 41)
+    base["off"] = (torch.arange(E + 1, device="cuda") * entries // E).to(torch.int32)
+
+    def case():
+        return {k_: v.clone() if torch.is_tensor(v) else v for k_, v in base.items()}
+
+    def same(o, want):
+        assert torch.equal(o.double(), want)
+
+    def reported(word):
+        with pytest.raises(InzgError) as e:
+            pool.device_status(_st())
+        assert e.value.status == 7 and word in str(e.value)
+
+    good = _grouped_want(base, E, entries, n)[0]
+    c = case()
+    c["off"][57] = 3
+    o, _ = _run_grouped(pool, t, c, E, entries, n, k, T_F32)
+    reported("offsets")
+    assert bool((o == CANARY).all())
+    for bad in ("in", "to"):
+        c = case()
+        c[bad][333] = c["a"].shape[0] if bad == "in" else -1
+        o, _ = _run_grouped(pool, t, c, E, entries, n, k, T_F32)
+        reported("row index")
+        want = good.clone()
+        want[base["to"][333].long()] = CANARY
+        same(o, want)
+    c = case()
+    c["off"] = c["off"].clamp(205, 6800).to(torch.int32)
+    o, _ = _run_grouped(pool, t, c, E, entries, n, k, T_F32)
+    same(o, _grouped_want(c, E, entries, n)[0])
+    c["off"].fill_(entries)
+    o, _ = _run_grouped(pool, t, c, E, entries, n, k, T_F32)
+    assert bool((o == CANARY).all())
+    c = case()
+    a = c["a"].float()
+    a[7, 100] = float("nan")
+    c["a"].copy_(a.to(DT[t]))
+    o, _ = _run_grouped(pool, t, c, E, entries, n, k, T_F32)
+    hit = base["to"][base["in"] == 7].long()
+    rest = torch.ones(len(good), dtype=torch.bool, device="cuda")
+    rest[hit] = False
+    assert bool(torch.isnan(o[hit]).all()) and torch.equal(o[rest].double(), good[rest])
+    pool.device_status(_st())
+
+    c, o = case(), torch.full_like(good, CANARY, dtype=torch.float32)
+    p = lambda x: x.data_ptr() if x is not None else None  # noqa: E731
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pool.grouped_matmul_device(t, E, n, k, c["a"].shape[0], entries, p(c["a"]), p(c["w"]), p(c["off"]), p(o), T_F32,
+                                   lda=c["a"].stride(0), ldw=c["w"].stride(0), a_scale_ptr=p(c["as"]), w_scale_ptr=p(c["ws"]),
+                                   in_rows_ptr=p(c["in"]), out_rows_ptr=p(c["to"]), out_scale_ptr=p(c["sc"]),
+                                   out_rows_n=c["out_rows_n"], stream=torch.cuda.current_stream().cuda_stream)
+    c["off"].copy_(_group_sizes(E, entries, _gen(8), True))
+    c["in"].copy_(c["in"].flip(0))
+    graph.replay()
+    torch.cuda.synchronize()
+    same(o, _grouped_want(c, E, entries, n)[0])
     pool.device_status(_st())
 
 
