@@ -321,7 +321,8 @@ INZG_EXPORT inzg_status inzg_matmul_q8(inzg_ctx *ctx, const inzg_matmul_q8_args 
 /* Products grouped by expert: for each group g and entry i in off[g] .. off[g + 1] - 1 (off on the device, ascending
  * from 0 or more to `entries` or less; groups may be empty)
  *   out[out_rows ? out_rows[i] : i][j] = (out_scale ? out_scale[i] : 1) * sum over k of a[in_rows ? in_rows[i] : i][k] * w[g][j][k]
- * with the block scales of inzg_matmul_q8 for INZG_T_E4M3; summed in fp32 and rounded once to out_type. a, w 16-byte
+ * with the block scales of inzg_matmul_q8 for INZG_T_E4M3; summed in fp32 and rounded once to out_type. (The tensor cores truncate
+ * their additions: they sum 128 k of e4m3 and 256 k of bf16 / f16, those sums are added rounding to nearest.) a, w 16-byte
  * aligned, their pitches multiples of 16 bytes. Entries outside the lists, and rows of out that none names, are left as they
  * were; an entry whose index is out of range is skipped and reported. A row of out named twice holds either value. */
 typedef struct {

@@ -5,7 +5,10 @@
 //   out[i][j] = scale_i * sum_b as[i][b] ws[j / 128][b] * (sum_{k in block b} a[i][k] w[g][j][k])
 //
 // The tensor core sums one block of 128 k in fp32 (TMEM); the block's two scales enter in the fold, which keeps the running
-// sum in fp32 registers: f = fma(dot_b, as * ws, f). bf16 / f16 have no scales and stay in TMEM over the whole k.
+// sum in fp32 registers: f = fma(dot_b, as * ws, f). bf16 / f16 have no scales, but each MMA truncates the sum that it leaves in
+// TMEM (16 k: some 0.4 * 2^-24 of it, always towards zero), so that a long k would drift: they leave TMEM every 256 k (kFold
+// steps) and are added up in fp32 registers, rounded to nearest. Error against 64 bits, fp32 results of random rows: 2.7e-6 at k = 2560
+// and 1.1e-5 at 10240 with the whole k in TMEM, 2.4e-7 and 2.6e-7 as it is, for 1.5 % of the time of 333 tokens' bf16 gate|up.
 //
 // Work item: 128 rows of w (the MMA's M, one TMEM lane each) x up to TN entries of one group (its N, rounded up to
 // 16). The weights are the M side because a decoding call has a row or two per expert: the MMA, the copies and the
@@ -48,6 +51,7 @@ struct GmmCfg {
     // item alone now takes some 320 cycles in both types, 18 KB at 57 bytes a cycle: what one SM gets from L2.
     static constexpr int kSub = TN <= 32 ? 2 : 1, kSubBytes = (GM + TN) * kGmmBytes;
     static constexpr int kStages = TN <= 32 ? 5 : 6, kStage = kSub * kSubBytes;
+    static constexpr int kFold = 4;                             // bf16 / f16: steps of k that stay in TMEM
     static constexpr int kSlot = kSub * TN;                     // TMEM columns of a slot
     static constexpr int kAcc = 512 / kSlot / kTeams, kGroup = kAcc / 2;  // slots per team: a team waits for its own alone, so it
                                                                 // is never two phases ahead
@@ -172,7 +176,8 @@ gmm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
                     for (int k0 = 0; k0 < steps; k0 += C::kSub) {
                         if (!(ok = mbar_wait(&S.full[slot.i], slot.parity, abort))) break;
                         const int subs = C::kSub == 1 ? 1 : min(C::kSub, steps - k0);
-                        const bool open = F8 || k0 == 0, close = F8 || k0 + C::kSub >= steps;
+                        const int in = F8 ? 0 : k0 % C::kFold;  // steps of the slot's sum before this one
+                        const bool open = in == 0, close = F8 || in + C::kSub == C::kFold || k0 + C::kSub >= steps;
                         if (open && mine.at.i % C::kGroup == 0) {
                             if (mine.given == 2) ok = mbar_wait(&S.acc_empty[team][mine.at.i / C::kGroup], mine.at.parity ^ 1, abort);
                             else mine.given++;
@@ -182,7 +187,7 @@ gmm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
                         for (int j = 0; j < subs; j++) {
                             const uint64_t da = desc0 + (uint64_t)((slot.i * C::kStage + j * C::kSubBytes) >> 4);
                             gmm_mma_stage<F8>(tmem + (team * NA + mine.at.i) * C::kSlot + (F8 ? j * TN : 0), da,
-                                              da + (GM * kGmmBytes >> 4), idesc, F8 || k0 + j == 0);
+                                              da + (GM * kGmmBytes >> 4), idesc, F8 || in + j == 0);
                         }
                         if (close) {
                             gmm_commit(&S.acc_full[team][mine.at.i]);
@@ -230,10 +235,11 @@ gmm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
             // item has, 20 steps of a dense product, us: 8 entries 10.2 -> 9.7, 24 entries as before; top-10 of 512, 4 tokens: 23.4 -> 23.2
             auto fold = [&](auto width) {
                 constexpr int W = decltype(width)::value;
-                for (int b0 = 0; b0 < (F8 ? steps : 1); b0 += kGmmKc) {
+                const int sums = F8 ? steps : (steps + C::kFold - 1) / C::kFold;
+                for (int b0 = 0; b0 < sums; b0 += kGmmKc) {
                     if (F8) ok = mbar_wait(&S.staged.p_full[team][ps.i], ps.parity, abort);
                     const float(&p)[kGmmKc][TN] = S.staged.p[team][ps.i][0];
-                    const int nb = F8 ? min(kGmmKc, steps - b0) : 1;
+                    const int nb = min(kGmmKc, sums - b0);
                     for (int b = 0; b < nb; b += F8 ? C::kSub : 1) {
                         const uint32_t from = lanes + acc.i * C::kSlot;
                         const bool two = F8 && b + 1 < nb;
@@ -278,8 +284,8 @@ gmm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
                                         if (F8) {
                                             add(to, &v[j * 4], *reinterpret_cast<const float4 *>(&p[b + q][c0 + j * 4]));
                                         } else {
-                                            to[0] = make_float2(v[j * 4], v[j * 4 + 1]);
-                                            to[1] = make_float2(v[j * 4 + 2], v[j * 4 + 3]);
+                                            to[0] = __fadd2_rn(make_float2(v[j * 4], v[j * 4 + 1]), to[0]);
+                                            to[1] = __fadd2_rn(make_float2(v[j * 4 + 2], v[j * 4 + 3]), to[1]);
                                         }
                                     }
                                 }

@@ -833,3 +833,46 @@ def test_layer_of_8bit_experts(n, kind):
     # v relative to the row) and e4m3 hidden values (2^-4 each, independent): in the 2-norm of a token below 2^-4
     rel = (z.double() - want_z).norm(dim=1) / want_z.norm(dim=1)
     assert float(rel.max()) <= 2.0 ** -4
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# Sums of bf16 / f16 products over a long k. What stands in TMEM is a chunk of 256 k: 16 MMAs, each adding 16 products to the sum and
+# truncating it (towards zero, by less than one step, 2u of the sum); the chunks' sums are added in fp32 to the nearest.
+
+
+@pytest.mark.parametrize("t", [T_BF16, T_F16])
+@pytest.mark.parametrize("m,gather", [(5, True), (300, False)])
+def test_grouped_long_sums_do_not_drift(pool, t, m, gather):
+    """Positive values, 200,008 k: every truncation of the running sum goes the same way. A chunk is off by at most one step per
+    product, 2 * 256 u of it, the chunks' sums by u per addition: (512 + k / 256 + 4) u = 1298 u. Truncated over the whole k the
+    sum would lose some 0.2 u per 16 k, 2400 u."""
+    E, n, k, g = 2, 130, 200_008, _gen(m)
+    a, w = (torch.rand(r, k, generator=g, device="cuda").add_(0.5).to(DT[t]) for r in (m, E * n))
+    off = torch.tensor([0, m // 2, m], dtype=torch.int32, device="cuda")
+    rows = torch.randperm(m, generator=g, device="cuda").to(torch.int32) if gather else None
+    o = torch.full((m, n), CANARY, device="cuda")
+    pool.grouped_matmul_device(t, E, n, k, m, m, a.data_ptr(), w.data_ptr(), off.data_ptr(), o.data_ptr(), T_F32,
+                               in_rows_ptr=rows.data_ptr() if gather else None, stream=_st())
+    for e in range(E):
+        i = slice(m // 2 * e, m // 2 if e == 0 else m)
+        x = a[rows[i].long()] if gather else a[i]
+        want = x.double() @ w[e * n:(e + 1) * n].double().t()
+        assert bool(((o[i].double() - want).abs() <= (512 + k // 256 + 4) * U * want).all())
+    pool.device_status(_st())
+
+
+@pytest.mark.parametrize("t", [T_BF16, T_F16])
+@pytest.mark.parametrize("m,k", [(5, 10_240), (300, 10_240), (40, 2568), (300, 2568), (300, 264)])
+def test_grouped_sums_have_no_bias(pool, t, m, k):
+    """Random signs: the mean error in the direction of the result, relative to the mean result. The running sum of a chunk grows
+    like the root of its MMAs: truncating each by at most 2u takes at most 2u * 16 * 2/3 = 21.3u of the chunk's size; rounding to the
+    nearest adds nothing on the mean, but a mean over m n results of an error of sqrt(k / 256 + 1) u each strays by
+    sqrt((k / 256 + 1) / (m n)) u, six of them allowed: under 1u here. Truncated over the whole k = 10240 it would be 160u."""
+    n, g = 640, _gen(k + m)
+    a, w = (torch.randn(r, k, generator=g, device="cuda").to(DT[t]) for r in (m, n))
+    off = torch.tensor([0, m], dtype=torch.int32, device="cuda")
+    o = torch.empty(m, n, device="cuda")
+    pool.grouped_matmul_device(t, 1, n, k, m, m, a.data_ptr(), w.data_ptr(), off.data_ptr(), o.data_ptr(), T_F32, stream=_st())
+    want = a.double() @ w.double().t()
+    bias = ((o.double() - want) * want.sign()).mean() / want.abs().mean()
+    assert abs(float(bias)) <= 22.3 * U
