@@ -300,7 +300,8 @@ INZG_EXPORT inzg_status inzg_silu_mul_q8(inzg_ctx *ctx, const inzg_silu_mul_q8_a
 /* The entries of n tokens' selections in order of expert, then slot t * topk + k: off [n_expert + 1] (the entries of
  * expert e are off[e] .. off[e + 1] - 1), rows (the token t of each entry), slots, w_out (w of each entry; NULL with w).
  * sel [n][topk]; a negative expert is on another rank and not listed, one >= n_expert is a device-side error and not
- * listed. n_expert <= INZG_MAX_GROUPS. */
+ * listed. The slots of entries that are not listed stay as they were in a product that follows, while inzg_combine adds
+ * all slots of a token: zero them first. n_expert <= INZG_MAX_GROUPS. */
 INZG_EXPORT inzg_status inzg_expert_lists(inzg_ctx *ctx, int n, int topk, int n_expert, const int32_t *sel,
                                           const float *w, int32_t *off, int32_t *rows, int32_t *slots, float *w_out,
                                           void *stream);

@@ -876,3 +876,55 @@ def test_grouped_sums_have_no_bias(pool, t, m, k):
     want = a.double() @ w.double().t()
     bias = ((o.double() - want) * want.sign()).mean() / want.abs().mean()
     assert abs(float(bias)) <= 22.3 * U
+
+
+def test_layer_with_absent_experts():
+    """The layer on one of two ranks: half of the experts are on the other one, a padded token has none at all. The slots held NaN and
+    are cleared before the down product; combine gives the sum of this rank's experts, 0 for the padded token."""
+    n, H, FF, E, K = 37, 2048, 640, 512, 10
+    from inferenz_b200 import synth
+    g = _gen(77)
+    quant = lambda r, k: (torch.randn(r, k, generator=g, device="cuda") * 120).clamp(-448, 448).to(F8)  # noqa: E731
+    scale = lambda *s: (torch.rand(*s, generator=g, device="cuda") + 0.5) / (120 * 45)  # noqa: E731
+    own = E // 2  # experts 256 to 511
+    wg, wd, sg, sd = quant(own * 2 * FF, H), quant(own * H, FF), scale(own, 2 * FF // 128, H // 128), scale(own, H // 128, FF // 128)
+    p = lambda t: t.data_ptr()  # noqa: E731
+    x, res = torch.randn(n, H, generator=g, device="cuda"), torch.randn(n, H, generator=g, device="cuda")
+    w = 1 + 0.1 * torch.randn(H, generator=g, device="cuda")
+    with MoePool(H, FF, E, K, max_tokens=64, n_layers=1, device=0) as pool:
+        pool.set_router(0, synth.router(0, E, H))
+        st = _st()
+        y, q, s = torch.empty_like(x), torch.empty(n, H, dtype=F8, device="cuda"), torch.empty(n, H // 128, device="cuda")
+        pool.rmsnorm_q8_device(n, H, T_F32, p(x), p(w), 1e-6, res_ptr=p(res), sum_ptr=p(res), y_ptr=p(y), q_ptr=p(q), s_ptr=p(s), stream=st)
+        sel, rw = torch.empty(n, K, dtype=torch.int32, device="cuda"), torch.empty(n, K, device="cuda")
+        pool.route_device(0, n, p(y), p(sel), p(rw), stream=st)
+        local = torch.where(sel >= own, sel - own, -1 - sel)
+        local[5] = -1
+        off, rows, slots = (torch.empty(m, dtype=torch.int32, device="cuda") for m in (own + 1, n * K, n * K))
+        lw = torch.empty(n * K, device="cuda")
+        pool.expert_lists_device(n, K, own, p(local), p(off), p(rows), p(slots), w_ptr=p(rw), w_out_ptr=p(lw), stream=st)
+        h = torch.full((n * K, 2 * FF), float("nan"), dtype=torch.bfloat16, device="cuda")
+        pool.grouped_matmul_device(T_E4M3, own, 2 * FF, H, n, n * K, p(q), p(wg), p(off), p(h), T_BF16, a_scale_ptr=p(s),
+                                   w_scale_ptr=p(sg), in_rows_ptr=p(rows), stream=st)
+        hq, hs = torch.empty(n * K, FF, dtype=F8, device="cuda"), torch.empty(n * K, FF // 128, device="cuda")
+        pool.silu_mul_q8_device(n * K, FF, T_BF16, p(h), q_ptr=p(hq), s_ptr=p(hs), stream=st)
+        out = torch.full((n * K, H), float("nan"), device="cuda")
+        out.zero_()
+        pool.grouped_matmul_device(T_E4M3, own, H, FF, n * K, n * K, p(hq), p(wd), p(off), p(out), T_F32, a_scale_ptr=p(hs),
+                                   w_scale_ptr=p(sd), out_rows_ptr=p(slots), out_scale_ptr=p(lw), stream=st)
+        z = torch.full((n, H), float("nan"), device="cuda")
+        pool.combine_device(n, p(out), p(z), stream=st)
+        pool.device_status(st)
+    listed = int(off[own])
+    assert 0 < listed == int((local >= 0).sum()) < n * K
+    want, mag = (torch.zeros(n, H, dtype=torch.float64, device="cuda") for _ in range(2))
+    hA, off_ = _deq(hq, hs), off.tolist()
+    for e in range(own):
+        i = torch.arange(off_[e], off_[e + 1], device="cuda")
+        if len(i):
+            D, sc = _deq_w(wd[e * H:(e + 1) * H], sd[e:e + 1], H)[0], lw[i].double()[:, None]
+            want.index_add_(0, rows[i].long(), hA[i] @ D.t() * sc)
+            mag.index_add_(0, rows[i].long(), hA[i].abs() @ D.abs().t() * sc)
+    # per entry (2 * 128 + 2 blocks + 4) u, the combine at most one u more per slot
+    assert bool(((z.double() - want).abs() <= (256 + 2 * (FF // 128) + 4 + K) * U * mag).all())
+    assert bool((z[5] == 0).all())
