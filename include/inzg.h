@@ -261,8 +261,11 @@ INZG_EXPORT inzg_status inzg_moe_block_hc(inzg_ctx *ctx, int layer, int n, float
  * written. Outputs must not overlap inputs except where said.
  *
  * Quantized rows: value[i][c] = q[i][c] * s[i][c / 128]. The quantizers set, per row and block of 128 columns,
- * s = max(max |v|, 2^-100) / 448 and q = e4m3(v / s), nearest, ties to even. A NaN stays a NaN in its place; a block
- * that holds an infinity has an infinite scale and no finite value.
+ * s = max(max |v|, 2^-100) / 448 and q = e4m3(v / s), nearest, ties to even. For inzg_silu_mul_q8 v is the result in fp32
+ * (y of INZG_T_F32) and v / s the quotient in fp32 (for a max |v| above 2^112 perhaps the neighbour of it). inzg_rmsnorm_q8
+ * takes v / s without the rounding of the row's factor, within 2^-22 of the exact quotient: that near a border of two e4m3
+ * values q may be either. A NaN stays a NaN in its place; a block that holds an infinity has an infinite scale and no finite
+ * value.
  *
  * Device-side checks (an expert id out of range, offsets that are not ascending within the entries, a row index out of
  * range) never read or write out of range; inzg_device_status reports them once (INZG_DEVICE_CHECK). */

@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(256, kSiluBlocks) silu_mul_q8_kernel(const inz
         if (A.y && left > 0) store_chunk<T, VEC>(static_cast<T *>(A.y) + r * A.ldy + c, left, v);
         if (A.q) {
             float s;
-            const uint2 q = quantize_chunk(v, s);
+            const uint2 q = quantize_chunk<true>(v, s);
             if (left > 0) {
                 store_q<VEC>(static_cast<uint8_t *>(A.q) + r * A.ldq + c, left, q);
                 if (first) A.s[r * A.lds + block] = s;

@@ -928,3 +928,28 @@ def test_layer_with_absent_experts():
     # per entry (2 * 128 + 2 blocks + 4) u, the combine at most one u more per slot
     assert bool(((z.double() - want).abs() <= (256 + 2 * (FF // 128) + 4 + K) * U * mag).all())
     assert bool((z[5] == 0).all())
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("n,cols,scale", [(20_000, 640, 1.0), (6000, 644, 1e-3), (3000, 300, 1e15), (3000, 640, 1e-14), (2000, 384, 1e-16),
+                                          (2000, 131, 1e-18)])
+def test_silu_quantizes_the_fp32_quotient(pool, n, cols, scale):
+    """q = e4m3(v / s) and s = max |v| / 448 bit for bit, with v the fp32 result and divisions in fp32; blocks of all magnitudes"""
+    g = _gen(cols)
+    x = torch.randn(n, 2 * cols, generator=g, device="cuda")
+    x[:, cols:] *= scale
+    y, q = torch.empty(n, cols, device="cuda"), torch.empty(n, cols, dtype=F8, device="cuda")
+    nb = (cols + 127) // 128
+    s = torch.empty(n, nb, device="cuda")
+    # gates below 1 in small cases take v down to the floor of the scale
+    x[:, :cols] *= min(1.0, scale)
+    pool.silu_mul_q8_device(n, cols, T_F32, x.data_ptr(), y_ptr=y.data_ptr(), q_ptr=q.data_ptr(), s_ptr=s.data_ptr(), stream=_st())
+    blocks = torch.nn.functional.pad(y, (0, nb * 128 - cols)).view(n, nb, 128)
+    floor = torch.tensor(2.0 ** -100, device="cuda")
+    most = torch.maximum(blocks.abs().amax(2), floor)
+    by = torch.full_like(most, 448.0)  # a tensor: by a number torch multiplies by the reciprocal
+    assert torch.equal(s, most / by)
+    want = (blocks / s[:, :, None]).to(F8).view(n, -1)[:, :cols]
+    assert torch.equal(q.view(torch.uint8), want.contiguous().view(torch.uint8))
