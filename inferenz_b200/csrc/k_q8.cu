@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(NCH > 2 ? 1024 : 512) rmsnorm_q8_kernel(const 
 // g / (1 + exp(-g)) of two values, in packed arithmetic. With x = g clamped to 88 and t = x log2 e rounded, exp(-x) =
 // 2^-t exp(t ln 2 - x); the last factor is within 2^-17 of 1, so 1 + (t ln 2 - x) stands for it and the relative error stays at a few
 // 2^-24 for large |x| too, where 2^-t alone loses |x| * 2^-24. Below -87.3 the divisor passes 2^126 and its estimated reciprocal
-// is 0 (and the quotient NaN for -infinity); the true value is less than 2^-119 there. A NaN passes through the last product.
+// is 0: silu_far is for gates below -87. A NaN passes through the last product.
 __device__ __forceinline__ float2 silu2(float2 g) {
     const float2 x = make_float2(fminf(fmaxf(g.x, -88.0f), 88.0f), fminf(fmaxf(g.y, -88.0f), 88.0f));
     const float2 t = __fmul2_rn(x, make_float2(1.4426950408889634f, 1.4426950408889634f));
@@ -112,10 +112,37 @@ __device__ __forceinline__ float2 silu2(float2 g) {
     return __fmul2_rn(g, make_float2(rcp_approx(d.x), rcp_approx(d.y)));
 }
 
+// g exp(g) u, which is g / (1 + exp(-g)) * u to within exp(-87) below -87: two factors take half of the exponential each, which alone
+// leaves fp32's normal range there while the product need not (u may be as large as 2^127), and what is below -160 comes last, when the
+// product is that small itself. Three exponentials (2 * 2^-24 each), four products.
+__device__ __noinline__ float silu_far(float g, float u) {
+    const float h = fmaxf(g, -160.0f), e = expf(0.5f * h);
+    return (g * e) * (u * e) * expf(g - h);
+}
+
+// the least of a chunk, NaN apart
+__device__ __forceinline__ float least_of(const Chunk<float> &c) {
+    float m = c.v[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) m = fminf(m, c.v[i]);
+    return m;
+}
+__device__ __forceinline__ float least_of(const Chunk<__nv_bfloat16> &c) {
+    const __nv_bfloat162 *p = reinterpret_cast<const __nv_bfloat162 *>(c.v);
+    const __nv_bfloat162 m = __hmin2(__hmin2(p[0], p[1]), __hmin2(p[2], p[3]));
+    return __bfloat162float(__hmin(m.x, m.y));
+}
+__device__ __forceinline__ float least_of(const Chunk<__half> &c) {
+    const __half2 *p = reinterpret_cast<const __half2 *>(c.v);
+    const __half2 m = __hmin2(__hmin2(p[0], p[1]), __hmin2(p[2], p[3]));
+    return __half2float(__hmin(m.x, m.y));
+}
+
 // A thread's slot: one chunk of one row; slots per row are rounded up to whole blocks of 128 columns. A thread goes on by
 // `step_rows` rows and `step_chunks` chunks, the grid's size in slots, and has the next slot's loads in flight. Four blocks per SM
 // (64 registers): 40960 x 640 bf16 26.1 us; 2 blocks 35.9, 3 28.8, 5 27.4, 6 28.0, 8 27.8; four with two slots ahead 29.1.
 constexpr int kSiluBlocks = 4;
+constexpr float kSiluFar = -87.0f;
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256, kSiluBlocks) silu_mul_q8_kernel(const inzg_silu_mul_q8_args A, uint32_t slots, uint32_t per_row,
                                                           uint32_t step_rows, uint32_t step_chunks) {
@@ -140,6 +167,7 @@ __global__ void __launch_bounds__(256, kSiluBlocks) silu_mul_q8_kernel(const inz
             gate[j] = to_f32(g.v[j]);
             v[j] = to_f32(u.v[j]);
         }
+        const bool far = least_of(g) < kSiluFar;
         i += gridDim.x * blockDim.x;
         row += step_rows;
         chunk += step_chunks;
@@ -153,6 +181,12 @@ __global__ void __launch_bounds__(256, kSiluBlocks) silu_mul_q8_kernel(const inz
             const float2 o = __fmul2_rn(silu2(make_float2(gate[j], gate[j + 1])), make_float2(v[j], v[j + 1]));
             v[j] = o.x;
             v[j + 1] = o.y;
+        }
+        if (__any_sync(0xffffffffu, far)) {  // seldom: once more from memory
+            const T *x = static_cast<const T *>(A.x) + r * A.ldx + c;
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (j < left && to_f32(x[j]) < kSiluFar) v[j] = silu_far(to_f32(x[j]), to_f32(x[cols + j]));
         }
         if (A.y && left > 0) store_chunk<T, VEC>(static_cast<T *>(A.y) + r * A.ldy + c, left, v);
         if (A.q) {

@@ -953,3 +953,52 @@ def test_silu_quantizes_the_fp32_quotient(pool, n, cols, scale):
     assert torch.equal(s, most / by)
     want = (blocks / s[:, :, None]).to(F8).view(n, -1)[:, :cols]
     assert torch.equal(q.view(torch.uint8), want.contiguous().view(torch.uint8))
+
+
+@pytest.mark.parametrize("t", [T_F32, T_BF16])
+def test_silu_of_far_negative_gates_beside_large_values(pool, t):
+    """gates from -80 to -190 with up values to 2^127: the result is a normal number although exp(-g) is none. Three exponentials of 2u
+    and four products: 10u; a result below the normal range is off by half a step of it (2^-150), and so may be a product before it, times
+    a factor below 1."""
+    dt, g = DT[t], _gen(3)
+    n, cols = 300, 256
+    x = torch.empty(n, 2 * cols, device="cuda")
+    x[:, :cols] = -80 - 110 * torch.rand(n, cols, generator=g, device="cuda")
+    x[:, :cols:7] = torch.randn(n, (cols + 6) // 7, generator=g, device="cuda")  # ordinary gates among them
+    x[:, cols:] = torch.exp2(127 * torch.rand(n, cols, generator=g, device="cuda")) * torch.where(
+        torch.rand(n, cols, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    x[0, :9] = torch.tensor([-87.0, -87.001, -86.999, -90.0, -100.0, -103.9, -176.0, -87.4, -88.7], device="cuda")
+    x[0, cols:cols + 9] = 1.5e38
+    x = x.to(dt)
+    y = torch.empty(n, cols, device="cuda", dtype=dt)
+    q, s = torch.empty(n, cols, dtype=F8, device="cuda"), torch.empty(n, cols // 128, device="cuda")
+    pool.silu_mul_q8_device(n, cols, t, x.data_ptr(), y_ptr=y.data_ptr(), q_ptr=q.data_ptr(), s_ptr=s.data_ptr(), stream=_st())
+    gate, up = x[:, :cols].double(), x[:, cols:].double()
+    want = gate * torch.exp(torch.minimum(gate, torch.zeros_like(gate))) / (1 + torch.exp(-gate.abs())) * up
+    assert float(want[0, 3].abs()) > 1  # what was 0
+    tiny = torch.finfo(dt).smallest_normal * torch.finfo(dt).eps
+    # an ordinary gate beside 2^127 leaves the type's range: infinite, and so is its block's scale
+    fits = want.abs() <= torch.finfo(dt).max
+    assert bool(((y.double() - want).abs() <= (half_step(dt) + 12 * U) * want.abs() * 1.01 + tiny)[fits].all())
+    assert torch.equal(y.double()[~fits], torch.sign(want[~fits]) * float("inf"))
+    whole = (want.abs() <= torch.finfo(torch.float32).max).view(n, -1, 128).all(2)
+    assert torch.equal(torch.isinf(s), ~whole) and int(whole.sum()) > n // 2
+    keep = whole[:, :, None].expand(n, cols // 128, 128).reshape(n, cols)
+    S = torch.where(whole, s, 1.0)
+    _check_quantized(torch.where(keep, q.float(), 0.0), torch.where(whole, S, float(2.0 ** -100) / 448), torch.where(keep, want, 0.0),
+                     torch.where(keep, 12 * U * want.abs() + 2.0 ** -149, 0.0))
+
+
+def test_silu_quantizes_around_infinities_and_nan(pool):
+    """a NaN stays in its place and leaves its block's scale; an infinite value makes its block's scale infinite and its values NaN"""
+    n, cols = 1, 384
+    x = torch.ones(n, 2 * cols, device="cuda")
+    x[0, 5], x[0, cols + 200] = float("nan"), float("inf")
+    x[0, 300] = -float("inf")  # (-inf) exp(-inf): NaN
+    y = torch.empty(n, cols, device="cuda")
+    q, s = torch.empty(n, cols, dtype=F8, device="cuda"), torch.empty(n, 3, device="cuda")
+    pool.silu_mul_q8_device(n, cols, T_F32, x.data_ptr(), y_ptr=y.data_ptr(), q_ptr=q.data_ptr(), s_ptr=s.data_ptr(), stream=_st())
+    nan = torch.isnan(q.float())[0].nonzero().flatten().tolist()
+    assert nan == [5] + list(range(128, 256)) + [300] and s[0, 1] == float("inf")
+    one = torch.tensor(float(y[0, 0]), device="cuda") / torch.tensor(448.0, device="cuda")
+    assert s[0, 0] == one and s[0, 2] == one and q[0, 0].float() == 448 and q[0, 383].float() == 448
