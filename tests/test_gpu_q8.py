@@ -1002,3 +1002,50 @@ def test_silu_quantizes_around_infinities_and_nan(pool):
     assert nan == [5] + list(range(128, 256)) + [300] and s[0, 1] == float("inf")
     one = torch.tensor(float(y[0, 0]), device="cuda") / torch.tensor(448.0, device="cuda")
     assert s[0, 0] == one and s[0, 2] == one and q[0, 0].float() == 448 and q[0, 383].float() == 448
+
+
+@pytest.mark.parametrize("t", [T_F32, T_BF16])
+@pytest.mark.parametrize("cols", [200, 2560, 8192, 16_388])
+@pytest.mark.parametrize("eps,place", [(0.0, "apart"), (1e-6, "res"), (1e-33, "x"), (1e-6, "apart")])
+def test_rmsnorm_of_rows_whose_squares_leave_the_range(pool, t, cols, eps, place):
+    """rows from 2^-140 to 2^124, ordinary ones among them and next to each other in a block's walk; the tolerances of any row (30u, the
+    factor being a power of two), and half a step of the smallest numbers for results down there"""
+    dt, g = DT[t], _gen(cols)
+    exps = [-140, 0, 124, -126, 64, 63, 62, 0, 60, 40, -40, -45, -46, -50, -64, -100, 80, 100, 120, 0] * 40  # several rows a block
+    n = len(exps)
+    x = (torch.randn(n, cols, generator=g, device="cuda").double() * torch.exp2(torch.tensor(exps, device="cuda").double())[:, None]).to(dt)
+    w = 1 + 0.2 * torch.randn(cols, generator=g, device="cuda")
+    res = (x.float() * torch.randn(n, cols, generator=g, device="cuda")).to(dt)  # of the row's size
+    res[2::20] = x[2::20] * 0.5  # but no sum past the range
+    eps32 = float(np.float32(eps))
+    h, v = _norm_want(x, res, w, eps32)
+    assert float(h.abs().max()) < 3.3e38
+    total = {"apart": torch.empty_like(x), "res": res, "x": x}[place]
+    y, q = torch.empty_like(x), torch.empty(n, cols, dtype=F8, device="cuda")
+    s = torch.empty(n, (cols + 127) // 128, device="cuda")
+    pool.rmsnorm_q8_device(n, cols, t, x.data_ptr(), w.data_ptr(), eps, res_ptr=res.data_ptr(), sum_ptr=total.data_ptr(),
+                           y_ptr=y.data_ptr(), q_ptr=q.data_ptr(), s_ptr=s.data_ptr(), stream=_st())
+    e, tiny = half_step(dt), torch.finfo(dt).smallest_normal * torch.finfo(dt).eps
+    assert bool(((total.double() - h).abs() <= (e + 2 * U) * h.abs() + tiny).all())  # the sum is that of the row as it is
+    zero = (h == 0).all(1) & (eps32 == 0)  # bf16 ends at 2^-133: such rows are zeros, 0 / 0
+    assert int(zero.sum()) == (40 if t == T_BF16 and eps32 == 0 else 0) and bool(torch.isnan(y[zero]).all())
+    y, q, s, v = y[~zero], q.view(torch.uint8)[~zero].view(F8), s[~zero], v[~zero]
+    assert bool(((y.double() - v).abs() <= (e + 30 * U) * v.abs() * (1 + e) + tiny).all())
+    _check_quantized(q, s, v, 30 * U * v.abs() + 2.0 ** -149)
+
+
+def test_rmsnorm_of_zero_infinite_and_nan_rows(pool):
+    """zeros with eps give zeros, without it 0 / 0; an infinity leaves zeros beside its own NaN; a NaN takes its row. Other rows are as
+    they are alone."""
+    cols, inf, nan = 2560, float("inf"), float("nan")
+    x = torch.randn(6, cols, generator=_gen(1), device="cuda")
+    x[1], x[2, 7], x[3, 9], x[4] = 0, inf, nan, x[4] * 1e30
+    w = torch.ones(cols, device="cuda")
+    for eps in (1e-6, 0.0):
+        y = torch.empty_like(x)
+        pool.rmsnorm_q8_device(6, cols, T_F32, x.data_ptr(), w.data_ptr(), eps, y_ptr=y.data_ptr(), stream=_st())
+        assert bool((y[1] == 0).all()) if eps else bool(torch.isnan(y[1]).all())
+        assert bool(torch.isnan(y[2, 7])) and int((y[2] == 0).sum()) == cols - 1 and bool(torch.isnan(y[3]).all())
+        rest = [0, 4, 5]
+        _, v = _norm_want(x[rest], None, w, float(np.float32(eps)))
+        assert bool(((y[rest].double() - v).abs() <= 31 * U * v.abs()).all())
