@@ -306,14 +306,12 @@ inzg_ctx *inzg_create(const inzg_config *cfg, inzg_status *status) {
     c->sh_tiles = dalloc<int32_t>(T / 16 + 2, ok);
     c->sh_meta = dalloc<int32_t>(16, ok);
     c->fused_cnt = dalloc<int32_t>(fused_counter_ints((int)E, 8, (int)H), ok);
-    if (ok && cudaMemset(c->fused_cnt, 0, sizeof(int32_t) * fused_counter_ints((int)E, 8, (int)H)) != cudaSuccess)
-        ok = false;
-    // status words start clear: a call whose logits are given runs no router that would clear them
-    if (ok && (cudaMemset(c->meta, 0, sizeof(int32_t) * 16) != cudaSuccess ||
-               cudaMemset(c->sh_meta, 0, sizeof(int32_t) * 16) != cudaSuccess))
-        ok = false;
     c->op_err = dalloc<int32_t>(1, ok);
-    if (ok && cudaMemset(c->op_err, 0, sizeof(int32_t)) != cudaSuccess) ok = false;
+    // Counters and status words start clear (a call whose logits are given runs no router that would clear them): on the context's own
+    // stream and waited for. The legacy stream's clears could come after the first calls, for which nothing on it waits.
+    auto clear = [&](void *p, size_t bytes) { return cudaMemsetAsync(p, 0, bytes, c->stream) == cudaSuccess; };
+    ok = ok && clear(c->fused_cnt, sizeof(int32_t) * fused_counter_ints((int)E, 8, (int)H)) && clear(c->meta, sizeof(int32_t) * 16) &&
+         clear(c->sh_meta, sizeof(int32_t) * 16) && clear(c->op_err, sizeof(int32_t)) && cudaStreamSynchronize(c->stream) == cudaSuccess;
     if (!ok) {
         free_scratch(c);
         cudaStreamDestroy(c->stream);

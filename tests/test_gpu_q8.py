@@ -1049,3 +1049,25 @@ def test_rmsnorm_of_zero_infinite_and_nan_rows(pool):
         rest = [0, 4, 5]
         _, v = _norm_want(x[rest], None, w, float(np.float32(eps)))
         assert bool(((y[rest].double() - v).abs() <= 31 * U * v.abs()).all())
+
+
+def test_a_new_context_is_clear_before_its_first_call(pool):
+    """A context made while the legacy stream is busy: its status words are cleared by then, not when that stream comes to it, so an
+    error that a first call records on another stream stands."""
+    stream = torch.cuda.Stream()
+    sel = torch.tensor([[0, 4], [2, 1]], dtype=torch.int32, device="cuda")
+    off, rows, slots = (torch.empty(5, dtype=torch.int32, device="cuda") for _ in range(3))
+    _lists(pool, torch.zeros_like(sel), 4)  # the library's kernels are loaded: that waits for the device
+    MoePool(2048, 640, 512, 10, max_tokens=16, n_layers=1, device=0).close()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(1_500_000_000)  # some 0.8 s on the legacy stream
+    with MoePool(2048, 640, 512, 10, max_tokens=16, n_layers=1, device=0) as pool:
+        busy = not torch.cuda.default_stream().query()
+        pool.expert_lists_device(2, 2, 4, sel.data_ptr(), off.data_ptr(), rows.data_ptr(), slots.data_ptr(), stream=stream.cuda_stream)
+        torch.cuda.synchronize()
+        with pytest.raises(InzgError) as e:
+            pool.device_status(stream.cuda_stream)
+        assert e.value.status == 7 and "expert id" in str(e.value)
+        pool.device_status(stream.cuda_stream)
+    if not busy:
+        pytest.skip("the legacy stream was idle again before the context was made")
