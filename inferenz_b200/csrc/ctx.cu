@@ -165,7 +165,7 @@ struct inzg_ctx {
     cudaStream_t capture_stream = nullptr;
     cudaStream_t side = nullptr;            // branch for the input quantization, joined before the experts
     cudaEvent_t fork = nullptr, join = nullptr;
-    int32_t *op_err = nullptr;  // error word of the 8-bit floating point operators, sticky until inzg_device_status
+    int32_t *op_err = nullptr;  // (in meta) error word of the 8-bit floating point operators, sticky until inzg_device_status
 };
 
 static const char *kStageNames[INZG_N_STAGES] = {"router_logits", "softmax_topk_route", "act_quant", "route",
@@ -212,7 +212,7 @@ static void free_scratch(inzg_ctx *c) {
                     c->gemm_units, c->gemm_tiles, c->upath, c->eexp, c->ew, c->GU, c->mo, c->dq64, c->dq256, c->dsb64,
                     c->ds256, c->xqe, c->xse, c->sh_cnt, c->sh_off, c->sh_first, c->sh_etok, c->sh_eslot,
                     c->sh_eexp, c->sh_upath, c->sh_units, c->sh_dec, c->sh_gemm, c->sh_tiles, c->sh_meta, c->sh_ew,
-                    c->cmask, c->fused_cnt, c->op_err};
+                    c->cmask, c->fused_cnt};
     for (void *p : ptrs)
         if (p) cudaFree(p);
 }
@@ -279,7 +279,8 @@ inzg_ctx *inzg_create(const inzg_config *cfg, inzg_status *status) {
     c->ccnt = dalloc<int32_t>(nchunk * E, ok);
     c->cmask = dalloc<uint64_t>(nchunk * E, ok);
     c->units = dalloc<int32_t>(E, ok);
-    c->meta = dalloc<int32_t>(16, ok);
+    c->meta = dalloc<int32_t>(16 + 1, ok);
+    c->op_err = c->meta ? c->meta + 16 : nullptr;  // behind them: inzg_device_status reads both in one copy
     c->dec_units = dalloc<int32_t>(E, ok);
     c->gemm_units = dalloc<int32_t>(E, ok);
     c->gemm_tiles = dalloc<int32_t>(NE / 16 + E, ok);
@@ -306,12 +307,11 @@ inzg_ctx *inzg_create(const inzg_config *cfg, inzg_status *status) {
     c->sh_tiles = dalloc<int32_t>(T / 16 + 2, ok);
     c->sh_meta = dalloc<int32_t>(16, ok);
     c->fused_cnt = dalloc<int32_t>(fused_counter_ints((int)E, 8, (int)H), ok);
-    c->op_err = dalloc<int32_t>(1, ok);
     // Counters and status words start clear (a call whose logits are given runs no router that would clear them): on the context's own
     // stream and waited for. The legacy stream's clears could come after the first calls, for which nothing on it waits.
     auto clear = [&](void *p, size_t bytes) { return cudaMemsetAsync(p, 0, bytes, c->stream) == cudaSuccess; };
-    ok = ok && clear(c->fused_cnt, sizeof(int32_t) * fused_counter_ints((int)E, 8, (int)H)) && clear(c->meta, sizeof(int32_t) * 16) &&
-         clear(c->sh_meta, sizeof(int32_t) * 16) && clear(c->op_err, sizeof(int32_t)) && cudaStreamSynchronize(c->stream) == cudaSuccess;
+    ok = ok && clear(c->fused_cnt, sizeof(int32_t) * fused_counter_ints((int)E, 8, (int)H)) && clear(c->meta, sizeof(int32_t) * (16 + 1)) &&
+         clear(c->sh_meta, sizeof(int32_t) * 16) && cudaStreamSynchronize(c->stream) == cudaSuccess;
     if (!ok) {
         free_scratch(c);
         cudaStreamDestroy(c->stream);
@@ -1008,10 +1008,11 @@ inzg_status inzg_device_status(inzg_ctx *c, void *stream) {
     if (!c) return INZG_BAD_ARG;
     cudaSetDevice(c->cfg.device);
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : c->stream;
-    int32_t meta[16];
+    int32_t meta[16 + 1];  // the status words and op_err
     cudaError_t e = cudaMemcpyAsync(meta, c->meta, sizeof(meta), cudaMemcpyDeviceToHost, st);
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
     if (e != cudaSuccess) return cuda_fail(c, e, "device_status");
+    const int32_t op_err = meta[16];
     const int code = meta[kMetaError] != kErrNone ? meta[kMetaError] : meta[kMetaRouterError];
     if (code != kErrNone) {
         char msg[96];
@@ -1025,14 +1026,11 @@ inzg_status inzg_device_status(inzg_ctx *c, void *stream) {
         if (e != cudaSuccess) return cuda_fail(c, e, "device_status");
         if (ep_err != kErrNone) return fail(c, INZG_TIMEOUT, "expert-parallel exchange: a peer did not arrive in time");
     }
-    int32_t op_err = 0;
-    e = cudaMemcpyAsync(&op_err, c->op_err, sizeof(op_err), cudaMemcpyDeviceToHost, st);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-    if (e == cudaSuccess && op_err != kErrNone) {
+    if (op_err != kErrNone) {
         e = cudaMemsetAsync(c->op_err, 0, sizeof(int32_t), st);
         if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+        if (e != cudaSuccess) return cuda_fail(c, e, "device_status");
     }
-    if (e != cudaSuccess) return cuda_fail(c, e, "device_status");
     if (op_err == kErrTimeout) return fail(c, INZG_TIMEOUT, "grouped_matmul: a device-side wait ran out");
     if (op_err != kErrNone)
         return fail(c, INZG_DEVICE_CHECK, op_err == kErrBadExpert ? "expert_lists: an expert id is out of range"

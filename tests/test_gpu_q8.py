@@ -1071,3 +1071,31 @@ def test_a_new_context_is_clear_before_its_first_call(pool):
         pool.device_status(stream.cuda_stream)
     if not busy:
         pytest.skip("the legacy stream was idle again before the context was made")
+
+
+def test_device_status_waits_once(pool):
+    """inzg_device_status, which callers of the older operators use after each step, is one copy and one wait: no slower than 1.5 times a
+    copy of 64 bytes by the runtime (two copies and two waits were twice that). The least of many batches, in turn."""
+    import ctypes
+    import time
+    src, dst = torch.zeros(64, dtype=torch.uint8, device="cuda"), torch.zeros(64, dtype=torch.uint8)
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def batch(call):
+        t = time.perf_counter()
+        for _ in range(100):
+            call()
+        return time.perf_counter() - t
+
+    handle = ctypes.c_void_p(st.cuda_stream)
+
+    def status():
+        assert lib.inzg_device_status(pool._ctx, handle) == 0
+
+    with torch.cuda.stream(st):
+        copies, statuses = [], []
+        for _ in range(30):
+            copies.append(batch(lambda: dst.copy_(src)))
+            statuses.append(batch(status))
+    assert min(statuses) <= 1.5 * min(copies), (min(statuses), min(copies))
