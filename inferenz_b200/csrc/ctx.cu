@@ -165,6 +165,7 @@ struct inzg_ctx {
     cudaStream_t capture_stream = nullptr;
     cudaStream_t side = nullptr;            // branch for the input quantization, joined before the experts
     cudaEvent_t fork = nullptr, join = nullptr;
+    int lists_cluster = 1;      // blocks of the largest cluster for inzg_expert_lists
     int32_t *op_err = nullptr;  // (in meta) error word of the 8-bit floating point operators, sticky until inzg_device_status
 };
 
@@ -323,7 +324,7 @@ inzg_ctx *inzg_create(const inzg_config *cfg, inzg_status *status) {
     gemv_set_attributes();
     gemm_tc_set_attributes();
     gmm_set_attributes();
-    lists_set_attributes();
+    c->lists_cluster = lists_set_attributes();
     c->have_tc = make_tma_map_i8(c->map_xqe.bytes, c->xqe, NE, H, 128) && make_tma_map_i8(c->map_dq.bytes, c->dq256, NE, FF, 128);
     for (int i = 0; i <= INZG_N_STAGES; i++) cudaEventCreate(&c->ev[i]);
     cudaStreamCreateWithFlags(&c->capture_stream, cudaStreamNonBlocking);
@@ -1335,9 +1336,10 @@ int inzg__router_view(const inzg_ctx *c, int layer, const void **router, int *de
 }
 
 // and for ops.cu
-void inzg__op_view(const inzg_ctx *c, int *device, int *num_sms, void **stream, int32_t **err) {
+void inzg__op_view(const inzg_ctx *c, int *device, int *num_sms, int *lists_cluster, void **stream, int32_t **err) {
     *device = c->cfg.device;
     *num_sms = c->num_sms;
+    *lists_cluster = c->lists_cluster;
     *stream = c->stream;
     *err = c->op_err;
 }

@@ -112,8 +112,10 @@ int launch_fused_decode(const LayerDev &L, int n, int K, const float *x, const f
 int launch_rmsnorm_q8(const inzg_rmsnorm_q8_args &args, int num_sms, cudaStream_t st);
 int launch_silu_mul_q8(const inzg_silu_mul_q8_args &args, int num_sms, cudaStream_t st);
 int launch_expert_lists(int n, int topk, int E, const int32_t *sel, const float *w, int32_t *off, int32_t *rows,
-                        int32_t *slots, float *w_out, int32_t *err, cudaStream_t st);
-void lists_set_attributes();
+                        int32_t *slots, float *w_out, int most_cluster, int32_t *err, cudaStream_t st);
+// on the current device: the blocks of the largest cluster that it can hold of the lists' kernel (16, 8 or 1), for most_cluster
+int lists_set_attributes();
+int lists_most_cluster(bool sixteen, bool eight);
 void gmm_set_attributes();
 // off null: one group of all entries (inzg_matmul_q8); -1: no tensor map for the operands
 int launch_grouped_matmul(const inzg_grouped_matmul_args &G, int num_sms, int32_t *err, cudaStream_t st);

@@ -2,7 +2,8 @@
 // without scratch in global memory; its shared-memory atomics only count and set bits, so the order is fixed.
 //
 // One block, or for more than 2048 entries a cluster of sixteen (past the portable eight, which took 14.1 us
-// where this takes 11.7: the scattered results leave through twice the SMs). A warp owns a contiguous run of the entries, a row of
+// where this takes 11.7: the scattered results leave through twice the SMs). Sixteen blocks of up to 208 KB of shared memory want as many
+// SMs of one GPC: where a device cannot hold them (lists_most_cluster) it is eight, or one. A warp owns a contiguous run of the entries, a row of
 // counters in shared memory, one per expert, and a row of lane masks: within a step of 32 entries the lanes set their bits in
 // their experts' masks (match.any, which does the same, goes through the distinct values one by one and was slower), so that
 //   place = (entries of smaller experts) + (own expert: earlier blocks, earlier warps, earlier steps, lower lanes)
@@ -17,7 +18,7 @@
 
 namespace inzg {
 
-constexpr int kListThreads = 1024, kListCluster = 16, kListCounters = 24576;  // counters of all warps, and as many masks: 192 KB
+constexpr int kListThreads = 1024, kListCounters = 24576;  // counters of all warps, and as many masks: 192 KB
 
 __device__ __forceinline__ void lists_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -138,17 +139,46 @@ expert_lists_kernel(const int32_t *__restrict__ sel, const float *__restrict__ w
     if (CLUSTER > 1) lists_cluster_sync();  // no block leaves while another may still read its totals
 }
 
-void lists_set_attributes() {
-    const int most = (2 * kListCounters + 2 * INZG_MAX_GROUPS) * (int)sizeof(int);
-    cudaFuncSetAttribute(expert_lists_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-    cudaFuncSetAttribute(expert_lists_kernel<kListCluster>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-    cudaFuncSetAttribute(expert_lists_kernel<kListCluster>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+constexpr int kListSmem = (2 * kListCounters + 2 * INZG_MAX_GROUPS) * (int)sizeof(int);  // of the longest lists
+
+static void lists_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute &at, int cluster, int threads, size_t smem, cudaStream_t st) {
+    cfg.gridDim = dim3(cluster);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = cluster;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+}
+
+// whether the device holds a cluster of so many blocks at their largest
+template <int CLUSTER>
+static bool lists_holds() {
+    const auto kernel = expert_lists_kernel<CLUSTER>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kListSmem) != cudaSuccess) return false;
+    if (CLUSTER > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at{};
+    lists_config(cfg, at, CLUSTER, kListThreads, kListSmem, nullptr);
+    int clusters = 0;
+    return cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess && clusters >= 1;
+}
+
+int lists_most_cluster(bool sixteen, bool eight) { return sixteen ? 16 : eight ? 8 : 1; }
+
+int lists_set_attributes() {
+    cudaFuncSetAttribute(expert_lists_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, kListSmem);
+    const bool sixteen = lists_holds<16>(), eight = lists_holds<8>();
+    cudaGetLastError();  // a size that the device refuses is no error of the caller's
+    return lists_most_cluster(sixteen, eight);
 }
 
 int launch_expert_lists(int n, int topk, int E, const int32_t *sel, const float *w, int32_t *off, int32_t *rows,
-                        int32_t *slots, float *w_out, int32_t *err, cudaStream_t st) {
+                        int32_t *slots, float *w_out, int most_cluster, int32_t *err, cudaStream_t st) {
     const int entries = n * topk;
-    const int cluster = entries > 2048 ? kListCluster : 1;
+    const int cluster = entries > 2048 ? most_cluster : 1;
     const int warps = std::max(1, std::min({kListThreads / 32, kListCounters / E, (entries + cluster * 32 - 1) / (cluster * 32)}));
     const size_t smem = sizeof(int) * (2 * (size_t)warps * E + 2 * (size_t)E);
     if (cluster == 1) {
@@ -156,17 +186,10 @@ int launch_expert_lists(int n, int topk, int E, const int32_t *sel, const float 
         return 1;
     }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(kListCluster);
-    cfg.blockDim = dim3(warps * 32);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
     cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = kListCluster;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, expert_lists_kernel<kListCluster>, sel, w, entries, topk, E, off, rows, slots, w_out, err);
+    lists_config(cfg, at, cluster, warps * 32, smem, st);
+    cudaLaunchKernelEx(&cfg, cluster == 16 ? expert_lists_kernel<16> : expert_lists_kernel<8>, sel, w, entries, topk, E, off, rows, slots,
+                       w_out, err);
     return 1;
 }
 

@@ -9,7 +9,8 @@
 #include "k_launch.h"
 
 // defined in ctx.cu (hidden)
-extern "C" void inzg__op_view(const inzg_ctx *ctx, int *device, int *num_sms, void **stream, int32_t **err);
+extern "C" void inzg__op_view(const inzg_ctx *ctx, int *device, int *num_sms, int *lists_cluster, void **stream,
+                              int32_t **err);
 extern "C" void inzg__set_error(inzg_ctx *ctx, const char *msg);
 
 namespace {
@@ -18,13 +19,13 @@ constexpr size_t kErrLen = 160;
 
 // the context's device for the duration of a call
 struct OpDevice {
-    int saved = -1, device = 0, num_sms = 0;
+    int saved = -1, device = 0, num_sms = 0, lists_cluster = 1;
     cudaStream_t st = nullptr;
     int32_t *err = nullptr;
     cudaError_t e = cudaSuccess;
     OpDevice(const inzg_ctx *c, void *stream) {
         void *own = nullptr;
-        inzg__op_view(c, &device, &num_sms, &own, &err);
+        inzg__op_view(c, &device, &num_sms, &lists_cluster, &own, &err);
         st = static_cast<cudaStream_t>(stream ? stream : own);
         e = cudaGetDevice(&saved);
         if (e == cudaSuccess && saved != device) e = cudaSetDevice(device);
@@ -79,7 +80,7 @@ inzg_status inzg_expert_lists(inzg_ctx *c, int n, int topk, int n_expert, const 
     const inzg_status s = inzg__check_expert_lists(n, topk, n_expert, sel, w, off, rows, slots, w_out, msg, sizeof(msg));
     if (s != INZG_OK) return refuse(c, s, msg);
     return run(c, stream, "expert_lists", [&](const OpDevice &d) {
-        return inzg::launch_expert_lists(n, topk, n_expert, sel, w, off, rows, slots, w_out, d.err, d.st);
+        return inzg::launch_expert_lists(n, topk, n_expert, sel, w, off, rows, slots, w_out, d.lists_cluster, d.err, d.st);
     });
 }
 
