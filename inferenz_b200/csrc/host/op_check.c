@@ -108,6 +108,7 @@ inzg_status inzg__check_matmul_q8(const inzg_matmul_q8_args *a, char *err, size_
     if (!a) REFUSE(INZG_BAD_ARG, "matmul_q8: no arguments");
     if (a->m < 0 || a->n <= 0 || a->k <= 0 || a->n > INT_MAX - 256 || a->k > INT_MAX - 256)
         REFUSE(INZG_BAD_ARG, "matmul_q8: bad m, n or k");
+    if (a->m > INT_MAX - 256) REFUSE(INZG_UNSUPPORTED, "matmul_q8: too many rows"); /* tiles are rounded up in 32 bits */
     if ((a->m / 16 + (int64_t)1) * (a->n / 128 + (int64_t)1) >= INT_MAX) REFUSE(INZG_UNSUPPORTED, "matmul_q8: too many tiles");
     if (a->m == 0) return INZG_OK;
     return check_product("matmul_q8", INZG_T_E4M3, a->n, a->n, a->k, a->m, a->a, a->lda, a->a_scale, a->lda_scale, a->w, a->ldw,
@@ -122,6 +123,7 @@ inzg_status inzg__check_grouped_matmul(const inzg_grouped_matmul_args *a, char *
         a->entries < 0 || a->out_rows_n < 0)
         REFUSE(INZG_BAD_ARG, "grouped_matmul: bad groups, n, k, a_rows, entries or out_rows_n");
     if (a->groups > INZG_MAX_GROUPS) REFUSE(INZG_UNSUPPORTED, "grouped_matmul: more than %d groups", INZG_MAX_GROUPS);
+    if (a->entries > INT_MAX - 256) REFUSE(INZG_UNSUPPORTED, "grouped_matmul: too many entries"); /* as for matmul_q8 */
     if ((a->entries / 16 + (int64_t)a->groups) * (a->n / 128 + (int64_t)1) >= INT_MAX)
         REFUSE(INZG_UNSUPPORTED, "grouped_matmul: too many tiles");
     if (a->entries == 0) return INZG_OK;

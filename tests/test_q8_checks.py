@@ -145,3 +145,18 @@ def test_struct_layouts_match_the_header(tmp_path):
         assert int(got[c]) == ctypes.sizeof(t)
         for f, _ in t._fields_:
             assert int(got[f"{c}.{f}"]) == getattr(t, f).offset
+
+
+M31 = 2**31 - 1
+
+
+@pytest.mark.parametrize("rows,want", [(M31, UNSUPPORTED), (M31 - 30, UNSUPPORTED), (M31 - 255, UNSUPPORTED), (M31 - 256, OK)])
+def test_rows_that_round_up_past_32_bits(checks, rows, want):
+    """the products number tiles of up to 128 entries in 32 bits: rounding the rows up to whole tiles must not pass them (the call was
+    accepted and computed nothing)"""
+    st, msg = _call(checks, "matmul_q8", _matmul(m=rows, n=1, k=16))
+    assert st == want and (st == OK or "too many rows" in msg)
+    st, msg = _call(checks, "grouped_matmul", _grouped(entries=rows, a_rows=rows, out_rows_n=rows, groups=1, n=1, k=16))
+    assert st == want and (st == OK or "too many entries" in msg)
+    st, msg = _call(checks, "grouped_matmul", _grouped(entries=rows, in_rows=P, out_rows=P, groups=1, n=1, k=16))
+    assert st == want and (st == OK or "too many entries" in msg)
