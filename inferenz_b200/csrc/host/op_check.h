@@ -18,6 +18,9 @@ inzg_status inzg__check_expert_lists(int n, int topk, int n_expert, const void *
 inzg_status inzg__check_matmul_q8(const inzg_matmul_q8_args *a, char *err, size_t len);
 inzg_status inzg__check_grouped_matmul(const inzg_grouped_matmul_args *a, char *err, size_t len);
 
+/* entries per tile of the grouped product's kernel for checked arguments: 32 or 128 */
+int inzg__grouped_matmul_tile(int type, int groups, int entries, int n, int num_sms);
+
 #ifdef __cplusplus
 }
 #endif

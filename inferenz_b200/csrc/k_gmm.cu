@@ -1,6 +1,6 @@
 // k_gmm.cu -- dense and grouped products of e4m3 rows with block scales, and of bf16 / f16 rows, on the 5th-generation
 // tensor cores (tcgen05.mma kind::f8f6f4 / kind::f16), sm_100a (inzg_matmul_q8, inzg_grouped_matmul): the kernel for few
-// entries per group, and the choice between it and the one for many (k_gmm_large.cu).
+// entries per group, and the launch of it or the one for many (k_gmm_large.cu).
 //
 //   out[i][j] = scale_i * sum_b as[i][b] ws[j / 128][b] * (sum_{k in block b} a[i][k] w[g][j][k])
 //
@@ -31,6 +31,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "host/op_check.h"
 #include "k_gmm.cuh"
 #include "k_launch.h"
 
@@ -419,22 +420,12 @@ int launch_grouped_matmul(const inzg_grouped_matmul_args &G, int num_sms, int32_
     // fp32 accumulators; e4m3 (0), bf16 (1) or f16 (0) operands, both K-major; M = 128
     const uint32_t fmt = G.type == INZG_T_BF16 ? 1u : 0u;
     A.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(GM >> 4) << 24);
-    // Which kernel, by the entries per group and by how many 32-entry items there are, taken to be one per 32 entries and half a one
-    // more per group (measured with k = 2048 and 2560, 32-entry tiles against 128-entry ones, us):
-    //   e4m3, 64 groups, n = 1280: 50 a group 44, 52; 62: 52, 53; 69: 55, 53; 80: 58, 52
-    //   e4m3, 512 groups, n = 640: 50 a group 150, 173; 62: 180, 190; 70: 192, 190
-    //   e4m3, one group, n = 2560: 128 entries 9.8, 16.5; 448: 14.4, 17.2; n = 10240: 96 entries 15.3, 17.2; 128: 18.8, 17.7
-    //   bf16, 64 groups, n = 1280: 40 a group 75, 82; 45: 80, 82; 52: 85, 81
-    //   bf16, one group, n = 1280: 192 entries 13, 19; n = 40960: 32 entries 42, 53; 64: 71, 57
-    // The entries of one group alone fill their tiles: past 32 its bf16 weights are streamed twice. A few items, up to one per SM
-    // (e4m3: two), are sooner done in small tiles whatever the groups.
-    const int64_t few = std::min<int64_t>(G.entries, (G.entries + 31LL) / 32 + (G.groups - 1) / 2) * A.nrb;
+    const bool small = inzg__grouped_matmul_tile(G.type, G.groups, G.entries, G.n, num_sms) == 32;
     if (G.type != INZG_T_E4M3) {
-        if (G.entries <= (G.groups > 1 ? 40 : 32) * (int64_t)G.groups || few <= num_sms || !g_wide_ok)
-            return gmm_launch<false, 32>(G, A, num_sms, st);
+        if (small || !g_wide_ok) return gmm_launch<false, 32>(G, A, num_sms, st);
         return gmm_launch<false, 128>(G, A, num_sms, st);
     }
-    if (G.entries <= 64 * (int64_t)G.groups || few <= 2 * num_sms || !g_large_ok) return gmm_launch<true, 32>(G, A, num_sms, st);
+    if (small || !g_large_ok) return gmm_launch<true, 32>(G, A, num_sms, st);
     return gmm_large_launch(G, A, num_sms, st);
 }
 

@@ -1099,3 +1099,70 @@ def test_device_status_waits_once(pool):
             copies.append(batch(lambda: dst.copy_(src)))
             statuses.append(batch(status))
     assert min(statuses) <= 1.5 * min(copies), (min(statuses), min(copies))
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# The tiles of 128 entries. The sizes are those of inzg__grouped_matmul_tile; test_q8_checks.py holds that they take these tiles.
+
+LONG_LISTS = [(T_E4M3, 2048, 2048 * 72, 9600), (T_BF16, 2048, 2048 * 42, 9600)]  # type, groups, entries, n
+RAGGED = [(T_E4M3, 3, 1700, 1301), (T_E4M3, 1, 1000, 1301), (T_BF16, 3, 1700, 1301), (T_F16, 1, 800, 1301)]
+
+
+@pytest.mark.parametrize("t,E,entries,n", LONG_LISTS)
+@pytest.mark.parametrize("gather", [False, True])
+def test_wide_tiles_past_the_list_of_items(pool, t, E, entries, n, gather):
+    """More items per SM than the 512 that a CTA lists: the roles search for the later ones. One or two entries of each group are listed, far
+    fewer than `entries`: 2048 tiles x 38 (or 75) row blocks over the SMs."""
+    g, k = _gen(n + gather), 16
+    f8 = t == T_E4M3
+    sizes = torch.randint(1, 3, (E,), generator=g, device="cuda")
+    off = torch.cat([torch.zeros(1, dtype=torch.int64, device="cuda"), sizes.cumsum(0)])
+    listed = int(off[-1])
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert E * ((n + 255) // 256 if f8 else (n + 127) // 128) // sms > 512 and listed < entries
+    a_rows = listed if gather else entries
+    a, w = _ints(a_rows, k, 16, DT[t], g), _ints(E * n, k, 16, DT[t], g)
+    sa, sw = (_pow2((a_rows, 1), g), _pow2((E, (n + 127) // 128, 1), g)) if f8 else (None, None)
+    rows = torch.full((entries,), -1, dtype=torch.int32, device="cuda")  # what is not listed is not read
+    rows[:listed] = torch.randint(0, a_rows, (listed,), generator=g, device="cuda")
+    to = torch.full((entries,), -1, dtype=torch.int32, device="cuda")
+    to[:listed] = torch.randperm(listed, generator=g, device="cuda")
+    o, off32 = torch.full((listed, n), CANARY, device="cuda"), off.to(torch.int32)
+    p = lambda x: x.data_ptr() if x is not None else None  # noqa: E731
+    pool.grouped_matmul_device(t, E, n, k, a_rows, entries, p(a), p(w), p(off32), p(o), T_F32, lda=16, ldw=16, a_scale_ptr=p(sa),
+                               w_scale_ptr=p(sw), in_rows_ptr=p(rows) if gather else None, out_rows_ptr=p(to), out_rows_n=listed, stream=_st())
+    pool.device_status(_st())
+    at = torch.arange(listed, device="cuda")
+    group = torch.searchsorted(off[1:], at, right=True)
+    src = rows[:listed].long() if gather else at
+    x = a.float()[src]
+    for c0 in range(0, n, 1200):  # small integers with powers of two: exact in fp32
+        c1 = min(n, c0 + 1200)
+        wc = (w.view(torch.uint8).view(E, n, -1)[:, c0:c1].contiguous().view(w.dtype) if f8 else w.unflatten(0, (E, n))[:, c0:c1]).float()
+        want = torch.bmm(wc[group], x[:, :, None])[:, :, 0]
+        if f8:
+            want = want * sa[src] * sw[group, :, 0].repeat_interleave(128, 1)[:, c0:c1]
+        assert torch.equal(o[to[:listed].long(), c0:c1], want)
+
+
+@pytest.mark.parametrize("t,E,entries,n", RAGGED)
+@pytest.mark.parametrize("out", TYPES)
+@pytest.mark.parametrize("gather,scatter,ld", [(True, True, 1304), (False, False, 1304), (True, False, 1312), (False, True, 1301)])
+def test_wide_tiles_of_ragged_columns(pool, t, E, entries, n, out, gather, scatter, ld):
+    """rows of out whose pitch is a whole number of 16-byte pieces while their width is none: the last piece is written in part, what is
+    behind it stays"""
+    k = 520
+    c = _grouped_case(t, E, entries, n, k, gather, scatter, 61)
+    o, ob = _rows(c["out_rows_n"], n, ld, DT[out])
+    assert o.data_ptr() % 16 == 0
+    p = lambda x: x.data_ptr() if x is not None else None  # noqa: E731
+    pool.grouped_matmul_device(t, E, n, k, c["a"].shape[0], entries, p(c["a"]), p(c["w"]), p(c["off"]), p(o), out,
+                               lda=c["a"].stride(0), ldw=c["w"].stride(0), ldo=ld, a_scale_ptr=p(c["as"]), w_scale_ptr=p(c["ws"]),
+                               in_rows_ptr=p(c["in"]), out_rows_ptr=p(c["to"]), out_scale_ptr=p(c["sc"]),
+                               out_rows_n=c["out_rows_n"], stream=_st())
+    want, _, wrote = _grouped_want(c, E, entries, n)
+    assert float(want.abs().max()) < 2.0 ** 20
+    assert torch.equal(o.double(), torch.where(wrote[:, None], want, torch.tensor(CANARY, dtype=torch.float64, device="cuda"))
+                       .to(DT[out]).double())
+    _behind_is_untouched(ob, o)
+    pool.device_status(_st())

@@ -160,3 +160,20 @@ def test_rows_that_round_up_past_32_bits(checks, rows, want):
     assert st == want and (st == OK or "too many entries" in msg)
     st, msg = _call(checks, "grouped_matmul", _grouped(entries=rows, in_rows=P, out_rows=P, groups=1, n=1, k=16))
     assert st == want and (st == OK or "too many entries" in msg)
+
+
+def _tile(checks, t, groups, entries, n, sms=148):
+    return checks.inzg__grouped_matmul_tile(t, groups, entries, n, sms)
+
+
+def test_which_tiles_a_product_takes(checks):
+    """few entries per group, or few items, take tiles of 32 entries; the tests of the wide tiles have sizes that take those"""
+    import test_gpu_q8 as gpu
+    for case in gpu.LONG_LISTS + gpu.RAGGED:
+        assert _tile(checks, *case) == 128
+    e4m3, bf16 = _lib.T_E4M3, _lib.T_BF16
+    assert [_tile(checks, e4m3, 512, m, 640) for m in (1, 320, 64 * 512, 64 * 512 + 1)] == [32, 32, 32, 128]
+    assert [_tile(checks, e4m3, 1, m, 10240) for m in (1, 96, 97, 4000)] == [32, 32, 128, 128]
+    assert [_tile(checks, bf16, 64, m, 1280) for m in (1, 40 * 64, 40 * 64 + 1)] == [32, 32, 128]
+    assert [_tile(checks, bf16, 1, m, 40960) for m in (32, 33)] == [32, 128] and _tile(checks, bf16, 1, 192, 1280) == 32
+    assert _tile(checks, e4m3, 2048, 2**31 - 256, 128) == 128 and _tile(checks, e4m3, 1, 2**31 - 256, 1) == 128
