@@ -726,7 +726,11 @@ def run_reference(args):
     # timed calls, so the run ends within minutes whatever --steps asks
     world = int(os.environ.get("WORLD_SIZE", "1"))
     n = 32 * world
-    cpu = cpu_reference("decode32", n, budget_s=90.0, steps=args.steps, warmup=max(args.warmup, 1))
+    try:
+        cpu = cpu_reference("decode32", n, budget_s=90.0, steps=args.steps, warmup=max(args.warmup, 1))
+    except FileNotFoundError as e:  # built from the reference's source, which is not here
+        print(json.dumps({"impl": "reference", "unavailable": f"the compiled reference is missing: {e}"}))
+        return
     line = {"metric": METRIC, "value": cpu["value"], "unit": "tokens/s", "impl": "reference",
             "n_gpus": world, "steps": args.steps, "warmup": args.warmup,
             "ms_per_step": cpu["ms_median"], "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
