@@ -138,14 +138,15 @@ inzg_status inzg__check_grouped_matmul(const inzg_grouped_matmul_args *a, char *
 }
 
 /* Which kernel, by the entries per group and by how many 32-entry items there are, taken to be one per 32 entries and half a one
- * more per group (measured with k = 2048 and 2560, 32-entry tiles against 128-entry ones, us):
+ * more per group (measured with k = 2048 and 2560, 32-entry tiles against 128-entry ones, us; bf16 while the whole k was summed in TMEM):
  *   e4m3, 64 groups, n = 1280: 50 a group 44, 52; 62: 52, 53; 69: 55, 53; 80: 58, 52
  *   e4m3, 512 groups, n = 640: 50 a group 150, 173; 62: 180, 190; 70: 192, 190
  *   e4m3, one group, n = 2560: 128 entries 9.8, 16.5; 448: 14.4, 17.2; n = 10240: 96 entries 15.3, 17.2; 128: 18.8, 17.7
  *   bf16, 64 groups, n = 1280: 40 a group 75, 82; 45: 80, 82; 52: 85, 81
  *   bf16, one group, n = 1280: 192 entries 13, 19; n = 40960: 32 entries 42, 53; 64: 71, 57
  * The entries of one group alone fill their tiles: past 32 its bf16 weights are streamed twice. A few items, up to one per SM
- * (e4m3: two), are sooner done in small tiles whatever the groups. */
+ * (e4m3: two), are sooner done in small tiles whatever the groups. `entries` is the caller's upper bound: a rank that lists few of
+ * them, or a few groups that have most of them, get the tiles of the mean. */
 int inzg__grouped_matmul_tile(int type, int groups, int entries, int n, int num_sms) {
     int64_t few = (entries + 31LL) / 32 + (groups - 1) / 2;
     if (few > entries) few = entries;

@@ -8,7 +8,8 @@
 // sum in fp32 registers: f = fma(dot_b, as * ws, f). bf16 / f16 have no scales, but each MMA truncates the sum that it leaves in
 // TMEM (16 k: some 0.4 * 2^-24 of it, always towards zero), so that a long k would drift: they leave TMEM every 256 k (kFold
 // steps) and are added up in fp32 registers, rounded to nearest. Error against 64 bits, fp32 results of random rows: 2.7e-6 at k = 2560
-// and 1.1e-5 at 10240 with the whole k in TMEM, 2.4e-7 and 2.6e-7 as it is, for 1.5 % of the time of 333 tokens' bf16 gate|up.
+// and 1.1e-5 at 10240 with the whole k in TMEM, 2.4e-7 and 2.6e-7 as it is (f16 3.5e-7). It costs 1 to 4 %: gate|up of 64 experts, 1280 x
+// 2560 bf16, one token 17.3 -> 18.0 us, 333 tokens 81.8 -> 82.5, 2000 tokens 222 -> 230.
 //
 // Work item: 128 rows of w (the MMA's M, one TMEM lane each) x up to TN entries of one group (its N, rounded up to
 // 16). The weights are the M side because a decoding call has a row or two per expert: the MMA, the copies and the
@@ -21,8 +22,8 @@
 //   warps 4-7   the entries' rows by index
 //   warps 8-15  fold and write, thread = a row of w. TN = 128 (bf16 / f16): all eight warps share an item, every other 32
 //               entries; TN = 32: the two warpgroups take the items in turn, so one writes while the other folds
-// Measured on B200, top-10 of 512 experts, gate|up 1280 x 2048 e4m3: 32 tokens 77 to 85 us (6 TB/s from DRAM), one token 11.5 us;
-// bf16 64 experts 1280 x 2560, 333 tokens 82 us (430 MB, 5.2 TB/s).
+// Measured on B200, back to back in CUDA graphs, top-10 of 512 experts, gate|up 1280 x 2048 e4m3: 32 tokens 73 to 85 us (6 TB/s from
+// DRAM), one token 10.5 us; bf16 64 experts 1280 x 2560, 333 tokens 82.5 us (430 MB, 5.2 TB/s), 2000 tokens 230 us.
 // Persistent: one CTA per SM walks the items; the offsets are turned into tile numbers by every CTA for itself, which
 // costs a read of off and a scan instead of a launch. Every mbarrier wait is bounded; on expiry the CTA records an
 // error, drains what it issued, frees its TMEM and returns.

@@ -11,8 +11,12 @@
 //   warps 4-7   the entries' rows by index
 //   warps 8-15  fold and write: thread = (entry, 128 of the 256 columns); the others hand registers over to these
 // Persistent, one CTA per SM; every mbarrier wait is bounded (k_gmm.cu).
-// Measured on B200: 4000 x 10240 x 2560 in 121 us (1730 TFLOP/s), bound by the chain of the fold between the two accumulators; 4096
-// tokens' down products (512 experts, 2048 x 640, fp32 slots) in 226 us (1.03 GB).
+// Measured on B200, back to back in CUDA graphs: 4000 x 10240 x 2560 in 121 us at best (1730 TFLOP/s), 126 to 134 in the median; 4096 tokens'
+// down products (512 experts, 2048 x 640, fp32 slots) in 224 us at best, 245 to 257 in the median (1.03 GB); their gate|up (1280 x 2048,
+// gathered, bf16) in 342 us at best, 407 in the median, 294 and 343 to 370 with rows in order. Eager calls take 142 and 258 us.
+// What bounds a step of 128 k is open: 830 cycles in the kernel, 572 for MMA, fold and hand-over measured alone, 862 for its 48 KB at the
+// 57 bytes a cycle that an SM alone got from L2 (k_gmm.cu), while a pair of CTAs that shares its copies gained 1 %. An item's
+// results take some 4000 cycles more, a fifth of a dense item, half of one with five steps, and are not overlapped with the next one's.
 #include <algorithm>
 
 #include "k_gmm.cuh"

@@ -6,8 +6,10 @@
 //
 // Both read each input once and write each output once: the row stays in registers (fp32) between the sum of squares
 // and the outputs, the block's largest value is a shuffle over 16 lanes, nothing passes through memory in between.
-// Measured on B200: norm of 4096 x 2560 bf16 with residual, y and e4m3 19.9 us (94.7 MB, 4.75 TB/s; 24.7 us without the next
-// row's loads in flight), one row 2.8 us; SiLU of 40960 x 640 bf16 26.1 to 26.9 us (131.9 MB, 5 TB/s).
+// Measured on B200, back to back in CUDA graphs: norm of 4096 x 2560 bf16 with residual, y and e4m3 19.5 us (94.7 MB, 4.85 TB/s; the
+// next row's loads in flight took it from 24.7 to 21.3 us when they came, one chunk per thread to 18.7), one row 2.2 us; SiLU of
+// 40960 x 640 bf16 28.0 us (131.9 MB, 4.7 TB/s). Eager calls from Python take 21.0 and 29.7 us. Rows that are not whole aligned chunks
+// go element by element: the norm with a pitch of 2563 49 to 72 us from one GPU to the next, SiLU of 40960 x 636 47 to 63 us.
 #include "k_launch.h"
 #include "k_q8.cuh"
 
@@ -249,7 +251,8 @@ __device__ __forceinline__ float least_of(const Chunk<__half> &c) {
 
 // A thread's slot: one chunk of one row; slots per row are rounded up to whole blocks of 128 columns. A thread goes on by
 // `step_rows` rows and `step_chunks` chunks, the grid's size in slots, and has the next slot's loads in flight. Four blocks per SM
-// (64 registers): 40960 x 640 bf16 26.1 us; 2 blocks 35.9, 3 28.8, 5 27.4, 6 28.0, 8 27.8; four with two slots ahead 29.1.
+// (64 registers): 40960 x 640 bf16 26.1 us; 2 blocks 35.9, 3 28.8, 5 27.4, 6 28.0, 8 27.8; four with two slots ahead 29.1. (28.0
+// since: 1.3 us for the exact quotient, 0.8 to look for gates below -87.)
 constexpr int kSiluBlocks = 4;
 constexpr float kSiluFar = -87.0f;
 template <class T, bool VEC>
@@ -323,7 +326,9 @@ static int norm_typed(const inzg_rmsnorm_q8_args &A, int num_sms, cudaStream_t s
     const int chunks = (A.cols + 7) / 8;
     const int nch = chunks <= 512 ? 1 : chunks <= 1024 ? 2 : 4;  // chunks per thread
     const int threads = ((chunks + nch - 1) / nch + 31) / 32 * 32;
-    const int per_sm = threads > 512 ? 1 : 1024 / threads;  // blocks that an SM holds with their next rows in registers
+    // Blocks per SM: as many as its registers hold with one chunk per thread (up to 64 registers). With two (91 to 112 registers) an SM holds
+    // one block of the one to three, and the others come after it.
+    const int per_sm = threads > 512 ? 1 : 1024 / threads;
     const int grid = (int)(A.n < (int64_t)num_sms * per_sm ? A.n : num_sms * per_sm);
     const bool late = A.sum && A.res && (A.sum == A.x || A.sum == A.res);
 #define INZG_NORM(NCH)                                                                                        \
