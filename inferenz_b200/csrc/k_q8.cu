@@ -10,6 +10,8 @@
 // next row's loads in flight took it from 24.7 to 21.3 us when they came, one chunk per thread to 18.7), one row 2.2 us; SiLU of
 // 40960 x 640 bf16 28.0 us (131.9 MB, 4.7 TB/s). Eager calls from Python take 21.0 and 29.7 us. Rows that are not whole aligned chunks
 // go element by element: the norm with a pitch of 2563 49 to 72 us from one GPU to the next, SiLU of 40960 x 636 47 to 63 us.
+#include <algorithm>
+
 #include "k_launch.h"
 #include "k_q8.cuh"
 
@@ -44,9 +46,10 @@ __device__ __forceinline__ bool norm_is_far(float ms) { return !(ms >= kMeanLeas
 // Those of the block's rows whose squares left fp32's range, or may have: h (and eps) are multiplied by a power of two that brings the
 // row's largest value, or the root of eps, to 1 to 4. After the other rows and from memory once more, over what was written for these
 // rows, so that the others do not wait for the decision: with h multiplied in their way 8192 columns took 64.7 us instead of
-// 56.5 and 10240 109 instead of 86. A row's ms is formed by the same operations in the same order as there.
+// 56.5 and 10240 109 instead of 86. `mark`: a bit for each of the block's rows; what x and res of the others hold by now may be sums.
+constexpr int kNormRows = 8192;  // rows of a block that can be marked; more take more launches
 template <class T, bool VEC>
-__device__ __forceinline__ void norm_far_rows(const inzg_rmsnorm_q8_args &A, float (&part)[32]) {
+__device__ __forceinline__ void norm_far_rows(const inzg_rmsnorm_q8_args &A, float (&part)[32], const uint32_t *mark) {
     const int cols = A.cols, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const int nch = (cols + 8 * blockDim.x - 1) / (8 * blockDim.x);  // every thread goes round as often: the quantizer shuffles
     auto reduce = [&](float v, auto op) {                            // over the block, in every thread
@@ -83,10 +86,13 @@ __device__ __forceinline__ void norm_far_rows(const inzg_rmsnorm_q8_args &A, flo
         }
         return __fdiv_rn(reduce(ss, [](float a, float b) { return a + b; }), (float)cols);
     };
+    __syncthreads();  // all marks are set
+    int at = -1;
 #pragma unroll 1
     for (int64_t row = blockIdx.x; row < A.n; row += gridDim.x) {
+        at++;
+        if (!(mark[at >> 5] >> (at & 31) & 1)) continue;
         float ms = mean(row, 1.0f) + A.eps;
-        if (!norm_is_far(ms)) continue;
         float most = __fsqrt_rn(A.eps), f = 1.0f;
 #pragma unroll 1
         for (int j = 0; j < nch; j++) {
@@ -123,6 +129,7 @@ template <class T, int NCH, bool VEC, bool LATE>
 __global__ void __launch_bounds__(NCH > 2 ? 1024 : 512) rmsnorm_q8_kernel(const inzg_rmsnorm_q8_args A) {
     constexpr bool AHEAD = NCH <= 2;
     __shared__ float part[2][32];
+    __shared__ uint32_t mark[kNormRows / 32];
     const int cols = A.cols, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     Chunk<T> x[AHEAD ? NCH : 1], r[AHEAD ? NCH : 1];
     auto load_part = [&](int64_t row, int j, int to) {
@@ -143,6 +150,9 @@ __global__ void __launch_bounds__(NCH > 2 ? 1024 : 512) rmsnorm_q8_kernel(const 
     if (AHEAD)
 #pragma unroll
         for (int j = 0; j < NCH; j++) load_w(j, w[AHEAD ? j : 0]);
+    const int rows = (A.n - 1 - (int)blockIdx.x) / (int)gridDim.x + 1;  // of the block
+    for (int i = threadIdx.x; i < (rows + 31) / 32; i += blockDim.x) mark[i] = 0;
+    __syncwarp();  // several warps pass a barrier before the first mark
     int flip = 0;
     bool far = false;  // whether one of the block's rows is
     for (int64_t row = blockIdx.x; row < A.n; row += gridDim.x, flip ^= 1) {
@@ -179,6 +189,10 @@ __global__ void __launch_bounds__(NCH > 2 ? 1024 : 512) rmsnorm_q8_kernel(const 
         const float ms = __fdiv_rn(ss, (float)cols) + A.eps;
         const bool far_row = norm_is_far(ms);  // the same for all threads of the block
         far |= far_row;
+        if (far_row && threadIdx.x == 0) {
+            const int at = (int)((row - blockIdx.x) / gridDim.x);
+            mark[at >> 5] |= 1u << (at & 31);
+        }
         if (LATE && !far_row) store_sum();
         const float rs = __frcp_rn(__fsqrt_rn(ms));
 #pragma unroll
@@ -202,7 +216,7 @@ __global__ void __launch_bounds__(NCH > 2 ? 1024 : 512) rmsnorm_q8_kernel(const 
             }
         }
     }
-    if (far) norm_far_rows<T, VEC>(A, part[0]);
+    if (far) norm_far_rows<T, VEC>(A, part[0], mark);
 }
 
 // g / (1 + exp(-g)) of two values, in packed arithmetic. With x = g clamped to 88 and t = x log2 e rounded, exp(-x) =
@@ -329,20 +343,32 @@ static int norm_typed(const inzg_rmsnorm_q8_args &A, int num_sms, cudaStream_t s
     // Blocks per SM: as many as its registers hold with one chunk per thread (up to 64 registers). With two (91 to 112 registers) an SM holds
     // one block of the one to three, and the others come after it.
     const int per_sm = threads > 512 ? 1 : 1024 / threads;
-    const int grid = (int)(A.n < (int64_t)num_sms * per_sm ? A.n : num_sms * per_sm);
+    const int64_t most = (int64_t)num_sms * per_sm * kNormRows;  // rows of a launch
     const bool late = A.sum && A.res && (A.sum == A.x || A.sum == A.res);
 #define INZG_NORM(NCH)                                                                                        \
     do {                                                                                                      \
-        if (vec && late) rmsnorm_q8_kernel<T, NCH, true, true><<<grid, threads, 0, st>>>(A);                  \
-        else if (vec) rmsnorm_q8_kernel<T, NCH, true, false><<<grid, threads, 0, st>>>(A);                    \
-        else if (late) rmsnorm_q8_kernel<T, NCH, false, true><<<grid, threads, 0, st>>>(A);                   \
-        else rmsnorm_q8_kernel<T, NCH, false, false><<<grid, threads, 0, st>>>(A);                            \
+        if (vec && late) rmsnorm_q8_kernel<T, NCH, true, true><<<grid, threads, 0, st>>>(P);                  \
+        else if (vec) rmsnorm_q8_kernel<T, NCH, true, false><<<grid, threads, 0, st>>>(P);                    \
+        else if (late) rmsnorm_q8_kernel<T, NCH, false, true><<<grid, threads, 0, st>>>(P);                   \
+        else rmsnorm_q8_kernel<T, NCH, false, false><<<grid, threads, 0, st>>>(P);                            \
     } while (0)
-    if (nch == 1) INZG_NORM(1);
-    else if (nch == 2) INZG_NORM(2);
-    else INZG_NORM(4);
+    int launches = 0;
+    for (int64_t done = 0; done < A.n; done += most, launches++) {
+        inzg_rmsnorm_q8_args P = A;
+        P.n = (int)std::min(A.n - done, most);
+        P.x = static_cast<const T *>(A.x) + done * A.ldx;
+        if (A.res) P.res = static_cast<const T *>(A.res) + done * A.ldres;
+        if (A.sum) P.sum = static_cast<T *>(A.sum) + done * A.ldsum;
+        if (A.y) P.y = static_cast<T *>(A.y) + done * A.ldy;
+        if (A.q) P.q = static_cast<uint8_t *>(A.q) + done * A.ldq;
+        if (A.s) P.s = A.s + done * A.lds;
+        const int grid = std::min(P.n, num_sms * per_sm);
+        if (nch == 1) INZG_NORM(1);
+        else if (nch == 2) INZG_NORM(2);
+        else INZG_NORM(4);
+    }
 #undef INZG_NORM
-    return 1;
+    return launches;
 }
 
 int launch_rmsnorm_q8(const inzg_rmsnorm_q8_args &args, int num_sms, cudaStream_t st) {

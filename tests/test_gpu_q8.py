@@ -1166,3 +1166,41 @@ def test_wide_tiles_of_ragged_columns(pool, t, E, entries, n, out, gather, scatt
                        .to(DT[out]).double())
     _behind_is_untouched(ob, o)
     pool.device_status(_st())
+
+
+@pytest.mark.parametrize("t", [T_F32, T_BF16])
+@pytest.mark.parametrize("cols", [200, 2560, 8192, 16_392])
+@pytest.mark.parametrize("place", ["res", "x", "apart"])
+def test_rmsnorm_in_place_beside_rows_taken_once_more(pool, t, cols, place):
+    """Rows that are taken once more among rows whose sum, written over x or res, would look like such a row if it were read again: just
+    below the range, or cancelling to 0 without eps. Each row's outputs are those of the row alone."""
+    dt, g, n = DT[t], _gen(cols + 1), 6000
+    kind = torch.randint(0, 4, (n,), generator=g, device="cuda")[:, None]
+    sign = torch.where(torch.rand(n, cols, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    near = 0.8 * (3.4e38 / cols) ** 0.5  # its squares' sum is 0.64 of the largest number, those of twice it are past it
+    one = torch.randn(n, cols, generator=g, device="cuda")
+    x = torch.where(kind == 0, one * 2.0 ** 100, torch.where(kind == 1, sign * near, one)).to(dt)
+    part = {"res": -2.0, "x": -0.5, "apart": -2.0}[place]  # x + (x + res), or (x + res) + res, is 0
+    res = torch.where(kind == 0, one * 2.0 ** 99, torch.where(kind == 1, 0.0, torch.where(kind == 2, x.float() * part, one))).to(dt)
+    w = 1 + 0.2 * torch.randn(cols, generator=g, device="cuda")
+    h, v = _norm_want(x, res, w, 0.0)
+    total = {"apart": torch.empty_like(x), "res": res, "x": x}[place]
+    y, q = torch.empty_like(x), torch.empty(n, cols, dtype=F8, device="cuda")
+    s = torch.empty(n, (cols + 127) // 128, device="cuda")
+    pool.rmsnorm_q8_device(n, cols, t, x.data_ptr(), w.data_ptr(), 0.0, res_ptr=res.data_ptr(), sum_ptr=total.data_ptr(),
+                           y_ptr=y.data_ptr(), q_ptr=q.data_ptr(), s_ptr=s.data_ptr(), stream=_st())
+    e, tiny = half_step(dt), torch.finfo(dt).smallest_normal * torch.finfo(dt).eps
+    assert bool(((total.double() - h).abs() <= (e + 2 * U) * h.abs() + tiny).all())
+    assert bool(((y.double() - v).abs() <= (e + 30 * U) * v.abs() * (1 + e) + tiny).all())
+    _check_quantized(q, s, v, 30 * U * v.abs() + 2.0 ** -149)
+
+
+def test_rmsnorm_of_more_rows_than_one_launch(pool):
+    """a block marks up to 8192 of its rows: more rows take more launches; the last ones far out"""
+    n, cols = 148 * 32 * 8192 + 77, 8
+    x = torch.ones(n, cols, device="cuda", dtype=torch.bfloat16)
+    x[-50:] = 2.0 ** 90
+    x[1000] = 2.0 ** 90
+    w, y = torch.ones(cols, device="cuda"), torch.zeros(n, cols, device="cuda", dtype=torch.bfloat16)
+    pool.rmsnorm_q8_device(n, cols, T_BF16, x.data_ptr(), w.data_ptr(), 0.0, y_ptr=y.data_ptr(), stream=_st())
+    assert bool((y == 1).all())
